@@ -82,4 +82,9 @@ from .eqt import (  # noqa: E402,F401
     layer_norm,
     lstm,
 )
+from .sequence import (  # noqa: E402,F401
+    cross_attention,
+    gated_scan,
+    relative_position_buckets,
+)
 from .adam import FusedAdam  # noqa: E402,F401

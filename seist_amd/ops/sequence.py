@@ -1,0 +1,338 @@
+"""Sequence mixing over long records: attention to the states of another
+length, with a learned position bias, and a gated linear recurrence.
+
+GPU: fused HIP kernels from ``seist_amd._C`` (cross_attention.hip,
+gated_scan.hip). CPU: plain fp32 PyTorch composites with identical
+semantics. Layouts are channels-first: (N, H, E, L) and (N, C, L).
+"""
+
+import functools
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import ext, use_native
+
+# the kernels' limits
+_MAX_DEPTH = 128
+_MAX_BUCKETS = 64
+_MAX_DISTANCE = 1024
+# a bias at or under this takes its pair out of the softmax
+_OUT = -1e30
+
+_DTYPES = (torch.float32, torch.bfloat16)
+
+
+def _refuse(op: str, what: str):
+    raise ValueError(f"{op}: {what}")
+
+
+def _check_lengths(op: str, name: str, lengths, like: torch.Tensor):
+    if lengths is None:
+        return None
+    if lengths.dim() != 1 or lengths.size(0) != like.size(0) \
+            or lengths.dtype not in (torch.int32, torch.int64) \
+            or lengths.device != like.device:
+        _refuse(op, f"{name} has to be ({like.size(0)},) int32 or int64 on "
+                    f"{like.device}, got {tuple(lengths.shape)} "
+                    f"{lengths.dtype} on {lengths.device}")
+    if lengths.dtype != torch.int32:
+        # a length past the end counts as the whole, one under zero as none
+        lengths = lengths.clamp(0, 2 ** 31 - 1).to(torch.int32)
+    return lengths.contiguous()
+
+
+def _rows_of_samples(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with unit stride along its last axis; other strides stay."""
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+# ---------------------------------------------------------------------------
+# learned relative position bias: distances to buckets
+# ---------------------------------------------------------------------------
+
+
+@functools.lru_cache(maxsize=None)
+def _bucket_thresholds(num_buckets: int, max_distance: int) -> list:
+    """Distances at which a side's buckets after the exact ones begin: the
+    m-th at exact * (max_distance / exact) ** (m / wide), rounded up, in
+    whole numbers so that no distance is ever off by a rounding."""
+    exact = num_buckets // 4
+    wide = num_buckets // 2 - exact
+    found = []
+    for m in range(1, wide):
+        least = exact ** (wide - m) * max_distance ** m
+        low, high = exact, max_distance
+        while low < high:
+            mid = (low + high) // 2
+            if mid ** wide >= least:
+                high = mid
+            else:
+                low = mid + 1
+        found.append(low)
+    return found
+
+
+def _check_buckets(op: str, num_buckets: int, max_distance: int):
+    if num_buckets % 2 or not 4 <= num_buckets <= _MAX_BUCKETS:
+        _refuse(op, f"an even number of buckets from 4 to {_MAX_BUCKETS} is "
+                    f"needed, got {num_buckets}")
+    if not num_buckets // 4 < max_distance <= _MAX_DISTANCE:
+        _refuse(op, f"max_distance has to be over {num_buckets // 4} and at "
+                    f"most {_MAX_DISTANCE}, got {max_distance}")
+
+
+def relative_position_buckets(distance: torch.Tensor, num_buckets: int,
+                              max_distance: int) -> torch.Tensor:
+    """Bucket of each signed distance (key position - query position).
+
+    Half of the buckets are for keys at or before the query, half for keys
+    after it. Of a half, the first ``num_buckets // 4`` stand for one distance
+    each; the rest widen geometrically up to ``max_distance``, and the last
+    holds everything from there on.
+    """
+    _check_buckets("relative_position_buckets", num_buckets, max_distance)
+    exact = num_buckets // 4
+    n = distance.abs()
+    steps = torch.tensor(_bucket_thresholds(num_buckets, max_distance),
+                         dtype=n.dtype, device=n.device)
+    at = torch.where(n < exact, n,
+                     exact + torch.bucketize(n, steps, right=True).to(n.dtype))
+    return at + (distance > 0).to(n.dtype) * (num_buckets // 2)
+
+
+# ---------------------------------------------------------------------------
+# attention to keys and values of another length
+# ---------------------------------------------------------------------------
+
+
+class _CrossAttention(torch.autograd.Function):
+    """Saves the output and one logarithm a query; scores are made again in
+    the backward pass (a per-query kernel for dq and the bias, a per-key
+    kernel for dk and dv)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, lengths, conf):
+        out, lse = ext().cross_attention_fwd(q, k, v, lengths, table, *conf,
+                                             True)
+        ctx.save_for_backward(q, k, v, table, lengths, out, lse)
+        ctx.conf = conf
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, lengths, out, lse = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dq, dk, dv, dtable = ext().cross_attention_bwd(
+            q, k, v, lengths, table, out, lse, _rows_of_samples(dout),
+            *ctx.conf, need[1] or need[2], need[3])
+        return (dq if need[0] else None, dk if need[1] else None,
+                dv if need[2] else None, dtable if need[3] else None, None,
+                None)
+
+
+def _cross_attention_plain(q, k, v, lengths, table, scale, key_step,
+                           query_start, max_distance):
+    N, H, E, Lq = q.shape
+    Hkv, Lk = k.size(1), k.size(3)
+    G = H // Hkv
+    qf = q.float().reshape(N, Hkv, G, E, Lq).transpose(-1, -2)
+    kf = k.float().unsqueeze(2)
+    vf = v.float().unsqueeze(2)
+    s = torch.matmul(qf, kf).reshape(N, H, Lq, Lk) * scale
+    if table is not None:
+        d = (torch.arange(Lk, device=q.device)[None, :] * key_step
+             - torch.arange(Lq, device=q.device)[:, None] - query_start)
+        bias = table.float()[:, relative_position_buckets(
+            d, table.size(1), max_distance)]
+        s = (s + bias).masked_fill(bias <= _OUT, -math.inf)
+    if lengths is not None:
+        hidden = torch.arange(Lk, device=q.device) >= lengths[:, None]
+        s = s.masked_fill(hidden[:, None, None, :], -math.inf)
+        vf = vf.masked_fill(hidden[:, None, None, None, :], 0.0)
+    # a query with no key left has no weights: zeros, and no gradient
+    none = (s == -math.inf).all(-1, keepdim=True)
+    p = torch.softmax(s.masked_fill(none, 0.0), -1).masked_fill(none, 0.0)
+    out = torch.matmul(p.reshape(N, Hkv, G, Lq, Lk), vf.transpose(-1, -2))
+    return out.transpose(-1, -2).reshape(N, H, E, Lq).to(q.dtype)
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                    kv_lengths: Optional[torch.Tensor] = None,
+                    bias_table: Optional[torch.Tensor] = None, *,
+                    key_step: int = 1, query_start: int = 0,
+                    max_distance: int = 128,
+                    scale: Optional[float] = None) -> torch.Tensor:
+    """softmax(scale * q^T k + bias) v^T to keys of any other length.
+
+    q: (N, H, E, Lq); k, v: (N, Hkv, E, Lk) with H a multiple of Hkv, query
+    head h reading key head h // (H // Hkv); E up to 128; all bf16 or all
+    fp32. Any strides; a copy is made only where the last axis is not
+    contiguous. Returns (N, H, E, Lq) in q's type. ``scale`` defaults to
+    1 / sqrt(E). Differentiable in q, k, v and ``bias_table``.
+
+    ``kv_lengths``: (N,), the keys of each record that count, from 0 to Lk;
+    nothing behind them is read into the result, NaN included.
+
+    ``bias_table``: (H, buckets) in q's type, added to the scores by the
+    bucket (:func:`relative_position_buckets`) of
+    ``j * key_step - (query_start + i)`` for key j and query i. ``key_step``
+    is the number of query positions a key stands for (the pooling ratio of
+    pooled keys), ``query_start`` the position of the first query (for queries
+    that come one at a time). An entry at or under -1e30, such as -inf or the
+    type's lowest value, takes its pairs out of the softmax.
+
+    A query with no key left gives zeros and no gradient.
+    """
+    op = "cross_attention"
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape \
+            or k.size(0) != q.size(0) or k.size(2) != q.size(2):
+        _refuse(op, "q (N, H, E, Lq) and k, v (N, Hkv, E, Lk) are needed, "
+                    f"got {tuple(q.shape)}, {tuple(k.shape)}, "
+                    f"{tuple(v.shape)}")
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        _refuse(op, "q, k and v have to be all float32 or all bfloat16, got "
+                    f"{q.dtype}, {k.dtype}, {v.dtype}")
+    if k.device != q.device or v.device != q.device:
+        _refuse(op, "q, k and v have to be on one device")
+    H, E = q.size(1), q.size(2)
+    if k.size(1) == 0 or H % k.size(1):
+        _refuse(op, f"{H} query heads cannot share {k.size(1)} key heads")
+    if not 1 <= E <= _MAX_DEPTH:
+        _refuse(op, f"heads of 1 to {_MAX_DEPTH} channels are needed, got "
+                    f"{E}")
+    lengths = _check_lengths(op, "kv_lengths", kv_lengths, q)
+    thresholds = []
+    if bias_table is not None:
+        if bias_table.dim() != 2 or bias_table.size(0) != H \
+                or bias_table.dtype != q.dtype \
+                or bias_table.device != q.device:
+            _refuse(op, f"bias_table has to be ({H}, buckets) {q.dtype} on "
+                        f"{q.device}, got {tuple(bias_table.shape)} "
+                        f"{bias_table.dtype} on {bias_table.device}")
+        _check_buckets(op, bias_table.size(1), max_distance)
+        if key_step < 1:
+            _refuse(op, f"key_step has to be 1 or more, got {key_step}")
+        if key_step * (k.size(3) + 128) >= 2 ** 30 \
+                or abs(query_start) + q.size(3) >= 2 ** 30:
+            _refuse(op, "positions have to stay under 2**30")
+        thresholds = _bucket_thresholds(bias_table.size(1), max_distance)
+    if scale is None:
+        scale = 1.0 / math.sqrt(E)
+    if not use_native(q):
+        return _cross_attention_plain(q, k, v, lengths, bias_table, scale,
+                                      key_step, query_start, max_distance)
+    q, k, v = _rows_of_samples(q), _rows_of_samples(k), _rows_of_samples(v)
+    if bias_table is not None:
+        bias_table = bias_table.contiguous()
+    conf = (scale, key_step, query_start, max_distance, thresholds)
+    if torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad or v.requires_grad
+            or (bias_table is not None and bias_table.requires_grad)):
+        return _CrossAttention.apply(q, k, v, bias_table, lengths, conf)
+    return ext().cross_attention_fwd(q, k, v, lengths, bias_table, *conf,
+                                     False)[0]
+
+
+# ---------------------------------------------------------------------------
+# gated linear recurrence
+# ---------------------------------------------------------------------------
+
+
+class _GatedScan(torch.autograd.Function):
+    """Saves the inputs and the fp32 state at the start of each chunk; the
+    backward pass makes the states in between again instead of reading h."""
+
+    @staticmethod
+    def forward(ctx, x, gate, state, lengths, reverse):
+        h, last, marks = ext().gated_scan_fwd(x, gate, state, lengths,
+                                              reverse, True)
+        ctx.save_for_backward(x, gate, lengths, marks)
+        ctx.reverse = reverse
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dlast):
+        x, gate, lengths, marks = ctx.saved_tensors
+        dx, dgate, dstate = ext().gated_scan_bwd(
+            x, gate, lengths, marks,
+            None if dh is None else dh.contiguous(),
+            None if dlast is None else dlast.contiguous(), ctx.reverse)
+        need = ctx.needs_input_grad
+        return (dx if need[0] else None, dgate if need[1] else None,
+                dstate if need[2] else None, None, None)
+
+
+def _gated_scan_plain(x, gate, state, lengths, reverse):
+    N, C, L = x.shape
+    gate = gate.float()
+    a, b = torch.sigmoid(gate), torch.sigmoid(-gate) * x.float()
+    valid = None
+    if lengths is not None:
+        valid = torch.arange(L, device=x.device) < lengths[:, None, None]
+        a = torch.where(valid, a, 1.0)
+        b = torch.where(valid, b, 0.0)
+    if reverse:
+        a, b = a.flip(-1), b.flip(-1)
+    h = x.new_zeros(N, C, dtype=torch.float32) if state is None else state
+    out = []
+    for t in range(L):
+        h = a[..., t] * h + b[..., t]
+        out.append(h)
+    hs = torch.stack(out, -1)
+    if reverse:
+        hs = hs.flip(-1)
+    if valid is not None:
+        hs = torch.where(valid, hs, 0.0)
+    return hs.to(x.dtype), h.clone()
+
+
+def gated_scan(x: torch.Tensor, gate: torch.Tensor,
+               state: Optional[torch.Tensor] = None,
+               lengths: Optional[torch.Tensor] = None,
+               reverse: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """h_t = sigmoid(gate_t) * h_{t-1} + (1 - sigmoid(gate_t)) * x_t.
+
+    x, gate: (N, C, L), both bf16 or both fp32, L at least 1; any strides, a
+    copy is made only where the last axis is not contiguous (so the two halves
+    of one projection can be given as they are). ``state``: the fp32 (N, C)
+    state before the first sample, zeros by default. Returns h (N, C, L) in
+    x's type and the fp32 state (N, C) after the last sample, which continues
+    a record that comes in pieces, down to one sample a call. Differentiable
+    in x, gate and state.
+
+    ``lengths``: (N,), the samples of each record that count; behind them h is
+    zero, the state stays, and nothing is read into the result. ``reverse``
+    runs from the last sample that counts to the first.
+    """
+    op = "gated_scan"
+    if x.dim() != 3 or gate.shape != x.shape or x.size(2) < 1:
+        _refuse(op, "x and gate of one shape (N, C, L), L at least 1, are "
+                    f"needed, got {tuple(x.shape)} and {tuple(gate.shape)}")
+    if x.dtype not in _DTYPES or gate.dtype != x.dtype:
+        _refuse(op, "x and gate have to be both float32 or both bfloat16, "
+                    f"got {x.dtype} and {gate.dtype}")
+    if gate.device != x.device:
+        _refuse(op, "x and gate have to be on one device")
+    if state is not None and (state.shape != x.shape[:2]
+                              or state.dtype != torch.float32
+                              or state.device != x.device):
+        _refuse(op, f"state has to be {tuple(x.shape[:2])} float32 on "
+                    f"{x.device}, got {tuple(state.shape)} {state.dtype} on "
+                    f"{state.device}")
+    lengths = _check_lengths(op, "lengths", lengths, x)
+    if not use_native(x):
+        return _gated_scan_plain(x, gate, state, lengths, reverse)
+    x, gate = _rows_of_samples(x), _rows_of_samples(gate)
+    if state is not None:
+        state = state.contiguous()
+    if torch.is_grad_enabled() and (
+            x.requires_grad or gate.requires_grad
+            or (state is not None and state.requires_grad)):
+        return _GatedScan.apply(x, gate, state, lengths, reverse)
+    h, last, _ = ext().gated_scan_fwd(x, gate, state, lengths, reverse, False)
+    return h, last

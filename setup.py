@@ -48,10 +48,14 @@ ext = CUDAExtension(
         os.path.join(HIP_DIR, "attention.hip"),
         os.path.join(HIP_DIR, "eqt.hip"),
         os.path.join(HIP_DIR, "loss.hip"),
+        os.path.join(HIP_DIR, "cross_attention.hip"),
+        os.path.join(HIP_DIR, "gated_scan.hip"),
     ],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
-        "nvcc": ["-O3", "-std=c++17"],
+        # packed fp32 instructions stay off: plain float code only
+        "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
+                 "-Xclang", "-packed-fp32-ops"],
     },
 )
 
