@@ -49,6 +49,7 @@ ext = CUDAExtension(
         os.path.join(HIP_DIR, "eqt.hip"),
         os.path.join(HIP_DIR, "loss.hip"),
         os.path.join(HIP_DIR, "cross_attention.hip"),
+        os.path.join(HIP_DIR, "cross_attention_bwd.hip"),
         os.path.join(HIP_DIR, "gated_scan.hip"),
     ],
     extra_compile_args={
