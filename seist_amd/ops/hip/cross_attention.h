@@ -305,6 +305,21 @@ __device__ __forceinline__ float bias_of(const Bias& b, int head, int d) {
   return v <= kOut ? -INFINITY : v * kLog2e;
 }
 
+// Where a distance's entry stands in a line of them. PADDED leaves out one
+// place in 16, so that lanes whose distances are 16 apart (keys pooled by 16)
+// do not all read the same banks.
+template <bool PADDED>
+__device__ __forceinline__ int line_at(int d) {
+  return PADDED ? d + (d >> 4) : d;
+}
+__host__ __device__ inline int line_floats(int max_distance, bool padded) {
+  return 2 * max_distance + 1 + (padded ? max_distance / 8 + 2 : 0);
+}
+// of distance 0 in such a line
+__host__ __device__ inline int line_middle(int max_distance, bool padded) {
+  return max_distance + (padded ? max_distance / 16 + 1 : 0);
+}
+
 // 32 columns of queries (or keys) against `span` positions of the other
 // sequence: whether every distance is past the last bucket's start. `least`
 // and `most` bound the distances; +1 and -1 say on which side.
@@ -312,14 +327,16 @@ __device__ __forceinline__ int beyond(const Bias& b, int least, int most) {
   return least >= b.max_distance ? 1 : most <= -b.max_distance ? -1 : 0;
 }
 
-// a head's bias by distance, -max_distance .. max_distance; `lane` of
-// `lanes` fill it
-template <typename T>
+// a head's bias by distance, -max_distance .. max_distance, at `line` for
+// distance 0; `lane` of `lanes` fill it
+template <typename T, bool PADDED>
 __device__ __forceinline__ void spread_bias(const Bias& b, int head,
                                             float* line, int lane,
                                             int lanes) {
-  for (int i = lane; i <= 2 * b.max_distance; i += lanes)
-    line[i] = bias_of<T>(b, head, i - b.max_distance);
+  for (int n = lane; n <= b.max_distance; n += lanes) {
+    line[line_at<PADDED>(-n)] = bias_of<T>(b, head, -n);
+    if (n > 0) line[line_at<PADDED>(n)] = bias_of<T>(b, head, n);
+  }
 }
 
 __device__ __forceinline__ int key_count(const Args& p, int n) {
@@ -327,13 +344,22 @@ __device__ __forceinline__ int key_count(const Args& p, int n) {
   return max(0, min(p.lengths[n], p.Lk));
 }
 
-// Consecutive workgroups go to the 8 dies in turn. Those that share keys and
-// values are consecutive here, so each die is given one run of them.
-__device__ __forceinline__ long spread_block() {
-  const long all = gridDim.x, at = blockIdx.x;
-  const long run = all / 8, rest = all % 8, die = at % 8;
-  return die * run + min(die, rest) + at / 8;
-}
+// Which work a workgroup has: its place among the `inner` workgroups of a
+// (record, key head) pair. Consecutive workgroups go to the 8 dies in turn;
+// a pair's share keys and values (or queries), so they are given to one die,
+// whose L2 then holds those, and neighbouring pairs to different dies, since
+// the heads of a long record are all long.
+struct Place {
+  int nh, at;
+  __device__ __forceinline__ Place(const Args& p, int inner) {
+    const unsigned block = blockIdx.x;
+    const unsigned even = (unsigned)(p.N * p.Hkv / 8) * 8 * inner;
+    const unsigned j = block < even ? block / 8 : block - even;
+    const unsigned k = j / inner;
+    at = j - k * inner;
+    nh = block < even ? k * 8 + block % 8 : even / inner + k;
+  }
+};
 
 // --- host --------------------------------------------------------------------
 
@@ -349,10 +375,13 @@ inline void launch(K kernel, long blocks, int threads, size_t lds, const Args& p
   SA_CHECK_HIP(hipGetLastError());
 }
 
-// positions of a staged tile
+// Positions of a staged tile: as many as 8 KB of it hold, from 32 to 128. A
+// tile has to be worked on for as long as the next one is on its way, so
+// heads of few channels need more positions.
 template <typename T, int ED>
 constexpr int tile_positions() {
-  return ED * sizeof(T) >= 512 ? 32 : 64;
+  constexpr int bytes = ED * sizeof(T);
+  return bytes >= 512 ? 32 : bytes > 64 ? 64 : 128;
 }
 
 template <typename F>

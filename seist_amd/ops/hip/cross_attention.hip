@@ -86,14 +86,13 @@ attend_kernel(Args p) {
   using M = Mma<T>;
   using Staged = Tile<T, ED, POS, 256>;
   constexpr int DB = (ED + 31) / 32;
-  constexpr int SUBS = POS / 32;
+  constexpr int STEP = POS < 64 ? POS : 64;  // keys worked on at once
+  constexpr int SUBS = STEP / 32;
   extern __shared__ char shared[];
 
-  long block = spread_block();
-  const int tile = block % p.tiles;
-  block /= p.tiles;
-  const int split = block % p.splits;
-  const int nh = block / p.splits;
+  const Place place(p, p.tiles * p.splits);
+  const int split = place.at / p.tiles, tile = place.at % p.tiles;
+  const int nh = place.nh;
   const int n = nh / p.Hkv, hk = nh % p.Hkv;
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
@@ -108,10 +107,10 @@ attend_kernel(Args p) {
   const int end = min(total, begin + p.per_split);
 
   float* line = (float*)(shared + 4 * Staged::kBytes) +
-                wave * (2 * p.bias.max_distance + 1) + p.bias.max_distance;
+                line_middle(p.bias.max_distance, false);
   float before = 0.0f, behind = 0.0f;
-  if (BIASED) {
-    spread_bias<T>(p.bias, head, line - p.bias.max_distance, lane, 64);
+  if (BIASED) {  // the workgroup's rows are one head's
+    spread_bias<T, false>(p.bias, head, line, tid, 256);
     before = bias_of<T>(p.bias, head, -p.bias.max_distance);
     behind = bias_of<T>(p.bias, head, p.bias.max_distance);
   }
@@ -154,70 +153,75 @@ attend_kernel(Args p) {
       ks.load(kb, at + POS, end, tid);
       vs.load(vb, at + POS, end, tid);
     }
-    float s[QB][SUBS][16];
+    if (first - g * p.pad >= p.Lq) continue;  // no query of this wave's
+#pragma unroll 1
+    for (int col = 0; col < POS && at + col < end; col += STEP) {
+      const int key0 = at + col;
+      float s[QB][SUBS][16];
 #pragma unroll
-    for (int b = 0; b < SUBS; ++b) {
-      f32x16 c[QB] = {};
+      for (int b = 0; b < SUBS; ++b) {
+        f32x16 c[QB] = {};
 #pragma unroll
-      for (int kk = 0; kk < ED / M::kDepth; ++kk) {
-        const auto a = M::template first<Staged::kStride>(kt, kk, 32 * b);
+        for (int kk = 0; kk < ED / M::kDepth; ++kk) {
+          const auto a = M::template first<Staged::kStride>(kt, kk, col + 32 * b);
 #pragma unroll
-        for (int o = 0; o < QB; ++o) c[o] = M::mul(a, q[o][kk], c[o]);
+          for (int o = 0; o < QB; ++o) c[o] = M::mul(a, q[o][kk], c[o]);
+        }
+#pragma unroll
+        for (int o = 0; o < QB; ++o)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[o][b][j] = c[o][j];
       }
-#pragma unroll
-      for (int o = 0; o < QB; ++o)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[o][b][j] = c[o][j];
-    }
-    if (at + POS > end) {
-#pragma unroll
-      for (int b = 0; b < SUBS; ++b)
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (at + 32 * b + M::seq(j, h) >= end)
-#pragma unroll
-            for (int o = 0; o < QB; ++o) s[o][b][j] = -INFINITY;
-    }
-    int side = 2;
-    if (BIASED) {
-      const int from = first - g * p.pad + p.bias.query_start;
-      side = beyond(p.bias, at * p.bias.key_step - (from + 32 * QB - 1),
-                    (at + POS - 1) * p.bias.key_step - from);
-    }
-    if (BIASED && side == 0) {
-#pragma unroll
-      for (int o = 0; o < QB; ++o) {
-        // the lane's own part of a distance; the rest is the wave's
-        const int d0 = (at + M::seq(0, h)) * p.bias.key_step -
-                       (i0 + 32 * o + p.bias.query_start);
+      if (key0 + STEP > end) {
 #pragma unroll
         for (int b = 0; b < SUBS; ++b)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int d = d0 + (32 * b + M::seq(j, 0)) * p.bias.key_step;
-            s[o][b][j] = fmaf(
-                s[o][b][j], scale,
-                line[max(-p.bias.max_distance, min(d, p.bias.max_distance))]);
-          }
-        weigh<SUBS, DB, true>(s[o], 1.0f, 0.0f, most[o], sum[o], acc[o]);
+          for (int j = 0; j < 16; ++j)
+            if (key0 + 32 * b + M::seq(j, h) >= end)
+#pragma unroll
+              for (int o = 0; o < QB; ++o) s[o][b][j] = -INFINITY;
       }
-    } else {
-      const float add = !BIASED ? 0.0f : side > 0 ? behind : before;
+      int side = 2;
+      if (BIASED) {
+        const int from = first - g * p.pad + p.bias.query_start;
+        side = beyond(p.bias, key0 * p.bias.key_step - (from + 32 * QB - 1),
+                      (key0 + STEP - 1) * p.bias.key_step - from);
+      }
+      if (BIASED && side == 0) {
 #pragma unroll
-      for (int o = 0; o < QB; ++o)
-        weigh<SUBS, DB, false>(s[o], scale, add, most[o], sum[o], acc[o]);
-    }
+        for (int o = 0; o < QB; ++o) {
+          // the lane's own part of a distance; the rest is the wave's
+          const int d0 = (key0 + M::seq(0, h)) * p.bias.key_step -
+                         (i0 + 32 * o + p.bias.query_start);
 #pragma unroll
-    for (int b = 0; b < SUBS; ++b) {
-      typename M::Right pr[QB];
+          for (int b = 0; b < SUBS; ++b)
 #pragma unroll
-      for (int o = 0; o < QB; ++o) M::right(pr[o], s[o][b]);
+            for (int j = 0; j < 16; ++j) {
+              const int d = d0 + (32 * b + M::seq(j, 0)) * p.bias.key_step;
+              s[o][b][j] = fmaf(
+                  s[o][b][j], scale,
+                  line[max(-p.bias.max_distance, min(d, p.bias.max_distance))]);
+            }
+          weigh<SUBS, DB, true>(s[o], 1.0f, 0.0f, most[o], sum[o], acc[o]);
+        }
+      } else {
+        const float add = !BIASED ? 0.0f : side > 0 ? behind : before;
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const auto a =
-            M::template second<Staged::kStride, ED>(vt, 32 * d, 32 * b);
+        for (int o = 0; o < QB; ++o)
+          weigh<SUBS, DB, false>(s[o], scale, add, most[o], sum[o], acc[o]);
+      }
 #pragma unroll
-        for (int o = 0; o < QB; ++o) acc[o][d] = M::mul(a, pr[o], acc[o][d]);
+      for (int b = 0; b < SUBS; ++b) {
+        typename M::Right pr[QB];
+#pragma unroll
+        for (int o = 0; o < QB; ++o) M::right(pr[o], s[o][b]);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const auto a =
+              M::template second<Staged::kStride, ED>(vt, 32 * d, col + 32 * b);
+#pragma unroll
+          for (int o = 0; o < QB; ++o) acc[o][d] = M::mul(a, pr[o], acc[o][d]);
+        }
       }
     }
   }
@@ -275,9 +279,8 @@ attend_few_kernel(Args p) {
   static_assert(ED * 32 * sizeof(float) <= BYTES, "a wave's sums fit");
   extern __shared__ char shared[];
 
-  long block = spread_block();
-  const int split = block % p.splits;
-  const int nh = block / p.splits;
+  const Place place(p, p.splits);
+  const int split = place.at, nh = place.nh;
   const int n = nh / p.Hkv, hk = nh % p.Hkv;
 
   const int lane = threadIdx.x & 63, h = lane >> 5;
@@ -493,13 +496,15 @@ __global__ __launch_bounds__(64) void attend_join_kernel(Args p) {
 
 template <typename T, int ED, int QB>
 void launch_attend(const Args& p, long blocks, hipStream_t stream) {
-  constexpr int POS = ED * QB > 128 ? 32 : tile_positions<T, ED>();
+  constexpr int POS = tile_positions<T, ED>();
   const size_t lds = 4 * Tile<T, ED, POS, 256>::kBytes;
-  if (p.bias.table)
-    launch(attend_kernel<T, ED, 1, POS, true>, blocks, 256,
-           lds + 16 * (2 * p.bias.max_distance + 1), p, stream);
-  else
-    launch(attend_kernel<T, ED, QB, POS, false>, blocks, 256, lds, p, stream);
+  if constexpr (QB == 1) {
+    if (p.bias.table)
+      return launch(attend_kernel<T, ED, 1, POS, true>, blocks, 256,
+                    lds + 4 * line_floats(p.bias.max_distance, false), p,
+                    stream);
+  }
+  launch(attend_kernel<T, ED, QB, POS, false>, blocks, 256, lds, p, stream);
 }
 
 }  // namespace attend
@@ -526,15 +531,16 @@ std::vector<at::Tensor> cross_attention_fwd(
   const long pairs = (long)p.N * p.Hkv;
   const bool few = (long)p.G * p.Lq <= 32;
   // two blocks of columns a wave where that still leaves every compute unit
-  // two workgroups; fp32 matrix products are too slow to wait for LDS
-  const bool twice = q.scalar_type() == at::kBFloat16 && !p.bias.table &&
+  // two workgroups and a SIMD two waves (heads up to 64); fp32 matrix
+  // products are too slow to wait for LDS
+  const bool twice = q.scalar_type() == at::kBFloat16 && p.E <= 64 && !p.bias.table &&
                      pairs * (p.G * (long)p.Lq / 256) >= 512;
   const int columns = twice ? 64 : 32;
-  p.pad = few ? p.Lq : round_up(p.Lq, columns);
+  // with a bias, a workgroup's rows are one head's
+  p.pad = few ? p.Lq : round_up(p.Lq, p.bias.table ? 4 * columns : columns);
   const long rows = (long)p.G * p.pad;
   p.tiles = few ? 1 : sa::ceil_div(rows, 4 * columns);
-  p.splits = cut(pairs * p.tiles, std::max(p.Lk, 1), few ? 128 : 64,
-                 &p.per_split);
+  p.splits = cut(pairs * p.tiles, std::max(p.Lk, 1), 128, &p.per_split);
   at::Tensor part, stat;
   if (p.splits > 1) {
     part = at::empty({p.splits * pairs * p.E * rows}, f32);
@@ -557,7 +563,7 @@ std::vector<at::Tensor> cross_attention_fwd(
         else
           launch(attend_few_kernel<T, ED, false>, blocks, 256, lds, p,
                  stream);
-      } else if constexpr (sizeof(T) == 2) {
+      } else if constexpr (sizeof(T) == 2 && ED <= 64) {
         if (twice) launch_attend<T, ED, 2>(p, blocks, stream);
         else launch_attend<T, ED, 1>(p, blocks, stream);
       } else {

@@ -5,19 +5,22 @@
 
 namespace attend {
 
-__device__ __forceinline__ int clamped(int d, int most) {
-  return max(-most, min(d, most)) + most;
-}
-
-// --- backward: dq, delta, dtable -------------------------------------------
-
-// LDS of a workgroup: two staged tiles and what stands behind them, where
-// the four waves' own columns pass through beforehand
+// LDS of a workgroup: two pairs of staged tiles and what stands behind them,
+// where the four waves' own columns pass through beforehand
 template <typename T, int ED>
 size_t backward_lds(size_t behind) {
   const size_t staged =
-      2 * Tile<T, ED, tile_positions<T, ED>(), 256>::kBytes + behind;
+      4 * Tile<T, ED, tile_positions<T, ED>(), 256>::kBytes + behind;
   return std::max<size_t>(staged, 4 * Columns<T, ED>::kBytes);
+}
+
+// the same for the kernel whose waves work in pairs, and what they hand over
+template <typename T, int ED>
+size_t deep_lds(size_t lines) {
+  constexpr int POS = tile_positions<T, ED>();
+  const size_t staged = 4 * Tile<T, ED, POS, 512>::kBytes + 16 * POS +
+                        (lines + 3) / 4 * 16 + 4 * (POS / 32) * 4096;
+  return std::max<size_t>(staged, 8 * Columns<T, ED>::kBytes);
 }
 
 // A wave's sums of ds by distance (one line for each half) and beyond the
@@ -54,50 +57,41 @@ __device__ __forceinline__ void fold_table(const Args& p, const float* lines,
 // query sums to zero over its keys; a delta made from the rounded output
 // would leave a remainder there that outgrows the entries, so bf16 walks the
 // keys once more beforehand for the delta that belongs to these p and dp.
-template <typename T, int ED, int NW, int POS, bool LINED, bool TABLE>
+template <typename T, int ED, int POS, bool LINED, bool TABLE>
 __global__ __launch_bounds__(
-    NW * 64, ED * (TABLE ? 2 : 1) * (sizeof(T) == 2 ? 2 : 8) <= 256 ? 2 : 1)
+    256, ED * (LINED ? 2 : 1) * (sizeof(T) == 2 ? 2 : 8) <= 256 ? 2 : 1)
 void attend_dq_kernel(Args p) {
   using M = Mma<T>;
-  using Staged = Tile<T, ED, POS, NW * 64>;
+  using Staged = Tile<T, ED, POS, 256>;
   constexpr int DB = (ED + 31) / 32;
-  constexpr int SUBS = POS / 32;
   constexpr bool TWICE = TABLE && sizeof(T) == 2;
   extern __shared__ char shared[];
-  T* kt = (T*)shared;
-  T* vt = (T*)(shared + Staged::kBytes);
 
-  long block = spread_block();
-  const int tile = block % p.tiles;
-  block /= p.tiles;
-  const int split = block % p.splits;
-  const int nh = block / p.splits;
+  const Place place(p, p.tiles * p.splits);
+  const int split = place.at / p.tiles, tile = place.at % p.tiles;
+  const int nh = place.nh;
   const int n = nh / p.Hkv, hk = nh % p.Hkv;
 
-  const int lane = threadIdx.x & 63, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = (tile * NW + wave) * 32 + (lane & 31);
-  const int g = min(row / p.pad, p.G - 1);
-  const int i = row - g * p.pad;
-  const bool live = i < p.Lq;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int first = (tile * 4 + wave) * 32;
+  const int g = min(first / p.pad, p.G - 1);
   const int head = hk * p.G + g;
-  const int position = p.bias.query_start + i;
-  const int wide = 2 * p.bias.max_distance + 1;
+  const int i0 = first - g * p.pad;  // the wave's first query
+  const int i = i0 + (lane & 31);
+  const bool live = i < p.Lq;
+  const int from = p.bias.query_start + i0;
+  const int far = p.bias.max_distance;
 
   const int total = key_count(p, n);
   const int begin = split * p.per_split;
   const int end = min(total, begin + p.per_split);
 
-  float* line = nullptr;
-  float* sums = nullptr;  // this half wave's ds by distance
-  float before = 0.0f, behind = 0.0f;  // and those beyond the last bucket
   typename M::Op q[ED / M::kDepth], go[ED / M::kDepth];
-  const int i0 = __builtin_amdgcn_readfirstlane(i);
-  const int head0 = __builtin_amdgcn_readfirstlane(head);
   T* own = (T*)shared + wave * (Columns<T, ED>::kBytes / sizeof(T));
-  own_columns<T, ED>(q, own, (const T*)p.q + n * p.qn + head0 * p.qh, p.qe,
+  own_columns<T, ED>(q, own, (const T*)p.q + n * p.qn + head * p.qh, p.qe,
                      p.E, i0, p.Lq);
-  own_columns<T, ED>(go, own, (const T*)p.dout + n * p.dn + head0 * p.dh,
+  own_columns<T, ED>(go, own, (const T*)p.dout + n * p.dn + head * p.dh,
                      p.de, p.E, i0, p.Lq);
   const long stat = ((long)n * p.H + head) * p.Lq + i;
   const float lse = live ? p.lse[stat] : INFINITY;
@@ -105,7 +99,7 @@ void attend_dq_kernel(Args p) {
   if (!TWICE) {
     typename M::Op o[ED / M::kDepth];
     own_columns<T, ED>(o, own,
-                       (const T*)p.o + ((long)n * p.H + head0) * p.E * p.Lq,
+                       (const T*)p.o + ((long)n * p.H + head) * p.E * p.Lq,
                        p.Lq, p.E, i0, p.Lq);
 #pragma unroll
     for (int kk = 0; kk < ED / M::kDepth; ++kk)
@@ -114,267 +108,484 @@ void attend_dq_kernel(Args p) {
         delta = fmaf(M::get(go[kk], j), M::get(o[kk], j), delta);
     delta = both_sum(delta);
   }
-  __syncthreads();
-  if (LINED) {
-    line = (float*)(shared + 2 * Staged::kBytes) + wave * (TABLE ? 3 : 1) * wide;
-    spread_bias<T>(p.bias, __builtin_amdgcn_readfirstlane(head), line, lane,
-                   64);
+  __syncthreads();  // the tiles come where the columns were
+
+  float* line = (float*)(shared + 4 * Staged::kBytes) +
+                line_middle(far, false);
+  float* lines = line + far + 1;  // the wave's ds by distance, a line a half
+  float before = 0.0f, behind = 0.0f;      // bias past the last bucket
+  float ds_before = 0.0f, ds_behind = 0.0f;
+  if (LINED) {  // the workgroup's rows are one head's
+    spread_bias<T, false>(p.bias, head, line, tid, 256);
+    before = bias_of<T>(p.bias, head, -far);
+    behind = bias_of<T>(p.bias, head, far);
     if (TABLE) {
-      for (int d = lane; d < 2 * wide; d += 64) line[wide + d] = 0.0f;
-      sums = line + (1 + h) * wide;
+      lines += wave * 2 * (2 * far + 1);
+      for (int d = lane; d < 2 * (2 * far + 1); d += 64) lines[d] = 0.0f;
     }
   }
+  float* sums = lines + h * (2 * far + 1) + far;
 
   f32x16 acc[DB] = {};
   const float scale = p.scale * kLog2e;
   const T* kb = (const T*)p.k + n * p.kn + hk * p.kh;
   const T* vb = (const T*)p.v + n * p.vn + hk * p.vh;
+  Staged ks, vs;
+  ks.place(p.ke, p.E, tid);
+  vs.place(p.ve, p.E, tid);
+  if (p.E < ED)
+    for (int b = 0; b < 4; ++b)
+      Staged::blank((T*)(shared + b * Staged::kBytes), p.E, tid);
 
 #pragma unroll 1
   for (int walk = TWICE ? 0 : 1; walk < 2; ++walk) {
-    Staged ks, vs;
-    ks.place(p.ke, p.E, threadIdx.x);
-    vs.place(p.ve, p.E, threadIdx.x);
     if (begin < end) {
-      Staged::blank(kt, p.E, threadIdx.x);
-      Staged::blank(vt, p.E, threadIdx.x);
-      ks.load(kb, begin, end, threadIdx.x);
-      vs.load(vb, begin, end, threadIdx.x);
+      ks.load(kb, begin, end, tid);
+      vs.load(vb, begin, end, tid);
     }
-    for (int at = begin; at < end; at += POS) {
-      __syncthreads();
-      ks.store(kt, p.E, threadIdx.x);
-      vs.store(vt, p.E, threadIdx.x);
+    if (TWICE) __syncthreads();  // the other walk's last tile
+    int buf = 0;
+    for (int at = begin; at < end; at += POS, buf ^= 1) {
+      T* kt = (T*)(shared + 2 * buf * Staged::kBytes);
+      T* vt = (T*)(shared + (2 * buf + 1) * Staged::kBytes);
+      ks.store(kt, p.E, tid);
+      vs.store(vt, p.E, tid);
       __syncthreads();
       if (at + POS < end) {
-        ks.load(kb, at + POS, end, threadIdx.x);
-        vs.load(vb, at + POS, end, threadIdx.x);
+        ks.load(kb, at + POS, end, tid);
+        vs.load(vb, at + POS, end, tid);
       }
-#pragma unroll
-      for (int b = 0; b < SUBS; ++b) {
+      if (i0 >= p.Lq) continue;  // no query of this wave's
+#pragma unroll 1
+      for (int col = 0; col < POS && at + col < end; col += 32) {
+        const int key0 = at + col;
         f32x16 c = {}, dp = {};
 #pragma unroll
         for (int kk = 0; kk < ED / M::kDepth; ++kk) {
-          c = M::mul(M::template first<Staged::kStride>(kt, kk, 32 * b),
-                     q[kk], c);
-          dp = M::mul(M::template first<Staged::kStride>(vt, kk, 32 * b),
+          c = M::mul(M::template first<Staged::kStride>(kt, kk, col), q[kk],
+                     c);
+          dp = M::mul(M::template first<Staged::kStride>(vt, kk, col),
                       go[kk], dp);
         }
+        int side = 2;
+        if (LINED)
+          side = beyond(p.bias, key0 * p.bias.key_step - (from + 31),
+                        (key0 + 31) * p.bias.key_step - from);
+        // the lane's own part of a distance; the rest is the wave's
+        const int d0 = (key0 + M::seq(0, h)) * p.bias.key_step - from -
+                       (lane & 31);
         float ds[16];
+        if (LINED && side == 0) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int key = at + 32 * b + M::seq(j, h);
-          float v = c[j] * scale;
-          if (LINED)
-            v += line[clamped(key * p.bias.key_step - position,
-                              p.bias.max_distance)];
-          const float e =
-              key < end ? __builtin_amdgcn_exp2f(v - lse) : 0.0f;
-          if (TWICE && walk == 0) delta = fmaf(e, dp[j], delta);
-          ds[j] = e * (dp[j] - delta);
+          for (int j = 0; j < 16; ++j) {
+            const int d = d0 + M::seq(j, 0) * p.bias.key_step;
+            ds[j] = fmaf(c[j], scale, line[max(-far, min(d, far))]) - lse;
+          }
+        } else {
+          const float off =
+              (!LINED ? 0.0f : side > 0 ? behind : before) - lse;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) ds[j] = fmaf(c[j], scale, off);
         }
-        if (TWICE && walk == 0) continue;
-        if (TABLE) {
+        if (key0 + 32 > end) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (key0 + M::seq(j, h) >= end) ds[j] = -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) ds[j] = __builtin_amdgcn_exp2f(ds[j]);
+        if (TWICE && walk == 0) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) delta = fmaf(ds[j], dp[j], delta);
+          continue;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) ds[j] *= dp[j] - delta;
+        if (TABLE && side == 0) {
           // the lanes of a half have different distances, and a wave's
           // additions reach LDS in order: the sums come out the same each
           // time
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const int key = at + 32 * b + M::seq(j, h);
-            const int d = key * p.bias.key_step - position;
-            const int where = clamped(d, p.bias.max_distance);
-            if (where == 0) before += ds[j];
-            else if (where == wide - 1) behind += ds[j];
-            else
-              __hip_atomic_fetch_add(sums + where, ds[j], __ATOMIC_RELAXED,
+            const int d = d0 + M::seq(j, 0) * p.bias.key_step;
+            ds_before += d <= -far ? ds[j] : 0.0f;
+            ds_behind += d >= far ? ds[j] : 0.0f;
+            if (d > -far && d < far)
+              __hip_atomic_fetch_add(sums + d, ds[j], __ATOMIC_RELAXED,
                                      __HIP_MEMORY_SCOPE_WORKGROUP);
           }
+        } else if (TABLE) {
+          float all = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) all += ds[j];
+          if (side > 0) ds_behind += all;
+          else ds_before += all;
         }
         typename M::Right pr;
         M::right(pr, ds);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
-          acc[d] = M::mul(M::template second<Staged::kStride, ED>(kt, 32 * d, 32 * b),
-                       pr, acc[d]);
+          acc[d] = M::mul(
+              M::template second<Staged::kStride, ED>(kt, 32 * d, col), pr,
+              acc[d]);
       }
     }
     if (TWICE && walk == 0) delta = both_sum(delta);
   }
   const int rows = p.G * p.pad;
   if (TABLE) {
-    __syncthreads();
-    fold_table(p, line + wide, before, behind,
-               p.dbias + (((long)n * p.H + head) * (p.pad / 32) + i / 32) *
+    wave_fence();
+    fold_table(p, lines, ds_before, ds_behind,
+               p.dbias + (((long)n * p.H + head) * (p.pad / 32) + i0 / 32) *
                              p.bias.buckets,
-               row - (lane & 31) < rows);
+               first < rows);
   }
-  if (row >= rows || !live) return;
-  if (p.delta && split == 0 && h == 0) p.delta[stat] = delta;
-  if (p.splits > 1) {
-    float* out = p.part +
-        (((long)split * p.N + n) * p.H + head) * p.E * p.Lq + i;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int e = 32 * d + 8 * (j / 4) + 4 * h + j % 4;
-        if (e < p.E) out[(long)e * p.Lq] = acc[d][j] * p.scale;
-      }
-    return;
-  }
-  T* out = (T*)p.out + ((long)n * p.H + head) * p.E * p.Lq + i;
-#pragma unroll
-  for (int d = 0; d < DB; ++d)
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int e = 32 * d + 8 * (j / 4) + 4 * h + j % 4;
-      if (e < p.E) out[(long)e * p.Lq] = (T)(acc[d][j] * p.scale);
-    }
-}
-
-// --- backward: dk, dv --------------------------------------------------------
-
-// A wave has 32 keys along its lanes and walks the queries of the heads that
-// read them, a workgroup staging 64 at a time: so the sum over shared heads
-// is made in registers.
-template <typename T, int ED, int NW, int POS, bool LINED>
-__global__ __launch_bounds__(NW * 64, ED * sizeof(T) <= 128 ? 2 : 1) void
-attend_dkv_kernel(Args p) {
-  using M = Mma<T>;
-  using Staged = Tile<T, ED, POS, NW * 64>;
-  constexpr int DB = (ED + 31) / 32;
-  constexpr int SUBS = POS / 32;
-  static_assert(POS <= NW * 64, "one thread stages one query's statistics");
-  extern __shared__ char shared[];
-  T* qt = (T*)shared;
-  T* dt = (T*)(shared + Staged::kBytes);
-  float* lses = (float*)(shared + 2 * Staged::kBytes);
-  float* deltas = lses + POS;
-  float* line = deltas + POS;
-
-  long block = spread_block();
-  const int tile = block % p.tiles;
-  block /= p.tiles;
-  const int split = block % p.splits;
-  const int nh = block / p.splits;
-  const int n = nh / p.Hkv, hk = nh % p.Hkv;
-
-  const int lane = threadIdx.x & 63, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int key = (tile * NW + wave) * 32 + (lane & 31);
-  const int total = key_count(p, n);
-  const bool live = key < total;
-
-  const int all = p.G * p.pad;
-  const int begin = split * p.per_split;
-  const int end = tile * NW * 32 < total ? min(all, begin + p.per_split) : 0;
-
-  typename M::Op k[ED / M::kDepth], v[ED / M::kDepth];
-  const int key0 = (tile * NW + wave) * 32;
-  if (begin < end) {
-    T* own = (T*)shared + wave * (Columns<T, ED>::kBytes / sizeof(T));
-    own_columns<T, ED>(k, own, (const T*)p.k + n * p.kn + hk * p.kh, p.ke,
-                       p.E, key0, total);
-    own_columns<T, ED>(v, own, (const T*)p.v + n * p.vn + hk * p.vh, p.ve,
-                       p.E, key0, total);
-    __syncthreads();
-  }
-
-  f32x16 dk[DB] = {}, dv[DB] = {};
-  const float scale = p.scale * kLog2e;
-  Staged qs, os;
-  qs.place(p.qe, p.E, threadIdx.x);
-  os.place(p.de, p.E, threadIdx.x);
-  float lse = INFINITY, delta = 0.0f;
-  auto fetch = [&](int row) {
-    const int g = row / p.pad, i = row - g * p.pad, head = hk * p.G + g;
-    qs.load((const T*)p.q + n * p.qn + head * p.qh, i, p.Lq, threadIdx.x);
-    os.load((const T*)p.dout + n * p.dn + head * p.dh, i, p.Lq, threadIdx.x);
-    lse = INFINITY;
-    delta = 0.0f;
-    if (threadIdx.x < POS && i + (int)threadIdx.x < p.Lq) {
-      const long at = ((long)n * p.H + head) * p.Lq + i + threadIdx.x;
-      lse = p.lse[at];
-      delta = p.delta[at];
-    }
-  };
-  if (begin < end) {
-    fetch(begin);
-    Staged::blank(qt, p.E, threadIdx.x);
-    Staged::blank(dt, p.E, threadIdx.x);
-  }
-  int lined = -1;
-  for (int row = begin; row < end; row += POS) {
-    const int g = row / p.pad, i = row - g * p.pad;
-    __syncthreads();
-    qs.store(qt, p.E, threadIdx.x);
-    os.store(dt, p.E, threadIdx.x);
-    if (threadIdx.x < POS) {
-      lses[threadIdx.x] = lse;
-      deltas[threadIdx.x] = delta;
-    }
-    if (LINED && g != lined) {
-      spread_bias<T>(p.bias, hk * p.G + g, line, threadIdx.x, NW * 64);
-      lined = g;
-    }
-    __syncthreads();
-    if (row + POS < end) fetch(row + POS);
-#pragma unroll
-    for (int b = 0; b < SUBS; ++b) {
-      f32x16 c = {}, dp = {};
-#pragma unroll
-      for (int kk = 0; kk < ED / M::kDepth; ++kk) {
-        c = M::mul(M::template first<Staged::kStride>(qt, kk, 32 * b), k[kk],
-                   c);
-        dp = M::mul(M::template first<Staged::kStride>(dt, kk, 32 * b), v[kk],
-                    dp);
-      }
-      float e[16], ds[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int at = 32 * b + M::seq(j, h);
-        float w = c[j] * scale;
-        if (LINED)
-          w += line[clamped(key * p.bias.key_step - p.bias.query_start - i -
-                                at,
-                            p.bias.max_distance)];
-        e[j] = __builtin_amdgcn_exp2f(w - lses[at]);
-        ds[j] = e[j] * (dp[j] - deltas[at]);
-      }
-      typename M::Right pr, dr;
-      M::right(pr, e);
-      M::right(dr, ds);
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        dv[d] = M::mul(M::template second<Staged::kStride, ED>(dt, 32 * d, 32 * b),
-                       pr, dv[d]);
-        dk[d] = M::mul(M::template second<Staged::kStride, ED>(qt, 32 * d, 32 * b),
-                       dr, dk[d]);
-      }
-    }
-  }
-  if (key >= p.Lk) return;
-  // a key that does not count has gone through with k = v = 0: its column
-  // holds numbers of no meaning
-  const long first = (long)nh * p.E * p.Lk + key;
-  const long whole = (long)p.N * p.Hkv * p.E * p.Lk;
+  if (first >= rows || !live) return;
+  if (split == 0 && h == 0) p.delta[stat] = delta;
+  const long to = ((long)n * p.H + head) * p.E * p.Lq + i;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const int e = 32 * d + 8 * (j / 4) + 4 * h + j % 4;
       if (e >= p.E) continue;
-      const long at = first + (long)e * p.Lk;
-      const float a = live ? dk[d][j] * p.scale : 0.0f;
-      const float b = live ? dv[d][j] : 0.0f;
-      if (p.splits > 1) {
-        p.part[split * whole + at] = a;
-        p.part[(p.splits + split) * whole + at] = b;
-      } else {
-        ((T*)p.dk)[at] = (T)a;
-        ((T*)p.dv)[at] = (T)b;
+      const float v = acc[d][j] * p.scale;
+      if (p.splits > 1)
+        p.part[(long)split * p.N * p.H * p.E * p.Lq + to +
+               (long)e * p.Lq] = v;
+      else
+        ((T*)p.out)[to + (long)e * p.Lq] = (T)v;
+    }
+}
+
+// --- backward: dk, dv --------------------------------------------------------
+
+// log2 p of SUBS blocks of 32 queries (rows, from position `from` on) for a
+// wave's 32 keys: scores, bias and the queries' logarithms
+template <typename T, int SUBS, bool LINED>
+__device__ __forceinline__ void log_weights(const Args& p,
+                                            f32x16 (&c)[SUBS],
+                                            const float* lses,
+                                            const float* line, float before,
+                                            float behind, int key0,
+                                            int from) {
+  using M = Mma<T>;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const float scale = p.scale * kLog2e;
+  const int far = p.bias.max_distance, step = p.bias.key_step;
+  int side = 2;
+  if (LINED)
+    side = beyond(p.bias, key0 * step - (from + 32 * SUBS - 1),
+                  (key0 + 31) * step - from);
+#pragma unroll
+  for (int b = 0; b < SUBS; ++b) {
+    if (LINED && side == 0) {
+      const int d0 =
+          (key0 + (lane & 31)) * step - from - 32 * b - M::seq(0, h);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 l = *(const f32x4*)(lses + 32 * b + M::seq(4 * g, h));
+#pragma unroll
+        for (int j = 4 * g; j < 4 * g + 4; ++j) {
+          const int d = d0 - M::seq(j, 0);
+          c[b][j] = fmaf(c[b][j], scale,
+                         line[line_at<true>(max(-far, min(d, far)))]) -
+                    l[j & 3];
+        }
+      }
+    } else {
+      const float add = !LINED ? 0.0f : side > 0 ? behind : before;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 l = *(const f32x4*)(lses + 32 * b + M::seq(4 * g, h));
+#pragma unroll
+        for (int j = 4 * g; j < 4 * g + 4; ++j)
+          c[b][j] =
+              fmaf(c[b][j], scale, LINED ? add - l[j & 3] : -l[j & 3]);
       }
     }
+  }
+}
+
+// What both kernels below do alike: a workgroup's 128 keys, 32 a wave, walk
+// the queries of the heads that read them, so that the sum over shared heads
+// is made in registers.
+template <typename T, int ED, int POS, int NT, bool LINED>
+struct Walk {
+  using Staged = Tile<T, ED, POS, NT>;
+  const Args& p;
+  int nh, n, hk, split, tile, tid, wave, total, begin, end;
+  char* shared;
+  float *stats, *line;  // (2, 2, POS) lse and delta; bias by distance
+  Staged qs, os;
+  float lse, delta, before, behind;
+  int lined, buf;
+  T *qt, *dt;
+  float *lses, *deltas;
+
+  __device__ __forceinline__ Walk(const Args& args, char* lds)
+      : p(args), shared(lds) {
+    const Place place(p, p.tiles * p.splits);
+    split = place.at / p.tiles;
+    tile = place.at % p.tiles;
+    nh = place.nh;
+    n = nh / p.Hkv;
+    hk = nh % p.Hkv;
+    tid = threadIdx.x;
+    wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    total = key_count(p, n);
+    begin = split * p.per_split;
+    end = tile * 128 < total ? min(p.G * p.pad, begin + p.per_split) : 0;
+    stats = (float*)(shared + 4 * Staged::kBytes);
+    line = stats + 4 * POS + line_middle(p.bias.max_distance, true);
+    lined = -1;
+    buf = 0;
+    before = behind = 0.0f;
+    qs.place(p.qe, p.E, tid);
+    os.place(p.de, p.E, tid);
+  }
+  __device__ __forceinline__ void fetch(int row) {
+    const int g = row / p.pad, i = row - g * p.pad, head = hk * p.G + g;
+    qs.load((const T*)p.q + n * p.qn + head * p.qh, i, p.Lq, tid);
+    os.load((const T*)p.dout + n * p.dn + head * p.dh, i, p.Lq, tid);
+    lse = INFINITY;
+    delta = 0.0f;
+    if (tid < POS && i + tid < p.Lq) {
+      const long at = ((long)n * p.H + head) * p.Lq + i + tid;
+      lse = p.lse[at];
+      delta = p.delta[at];
+    }
+  }
+  __device__ __forceinline__ void start() {
+    if (p.E < ED)
+      for (int b = 0; b < 4; ++b)
+        Staged::blank((T*)(shared + b * Staged::kBytes), p.E, tid);
+    fetch(begin);
+  }
+  // puts down the queries row.. and starts on the next ones
+  __device__ __forceinline__ void next(int row) {
+    qt = (T*)(shared + 2 * buf * Staged::kBytes);
+    dt = (T*)(shared + (2 * buf + 1) * Staged::kBytes);
+    lses = stats + 2 * buf * POS;
+    deltas = lses + POS;
+    buf ^= 1;
+    qs.store(qt, p.E, tid);
+    os.store(dt, p.E, tid);
+    if (tid < POS) {
+      lses[tid] = lse;
+      deltas[tid] = delta;
+    }
+    if (LINED) {
+      const int g = row / p.pad;
+      if (g != lined) {  // the next head's
+        __syncthreads();
+        spread_bias<T, true>(p.bias, hk * p.G + g, line, tid, NT);
+        before = bias_of<T>(p.bias, hk * p.G + g, -p.bias.max_distance);
+        behind = bias_of<T>(p.bias, hk * p.G + g, p.bias.max_distance);
+        lined = g;
+      }
+    }
+    __syncthreads();
+    if (row + POS < end) fetch(row + POS);
+  }
+  // a wave's columns of dk or dv
+  template <int DB>
+  __device__ __forceinline__ void store(const f32x16 (&acc)[DB], T* out,
+                                        int half, int key, float by) const {
+    if (key >= p.Lk) return;
+    // a key that does not count has gone through with k = v = 0: its column
+    // holds numbers of no meaning
+    const bool live = key < total;
+    const int h = (tid & 63) >> 5;
+    const long to = (long)nh * p.E * p.Lk + key;
+    float* part = p.part + ((long)half * p.splits + split) * p.N * p.Hkv *
+                               p.E * p.Lk;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int e = 32 * d + 8 * (j / 4) + 4 * h + j % 4;
+        if (e >= p.E) continue;
+        const float v = live ? acc[d][j] * by : 0.0f;
+        if (p.splits > 1) part[to + (long)e * p.Lk] = v;
+        else out[to + (long)e * p.Lk] = (T)v;
+      }
+  }
+};
+
+template <typename T, int ED, int POS, bool LINED>
+__global__ __launch_bounds__(256, 2) void attend_dkv_kernel(Args p) {
+  using M = Mma<T>;
+  using W = Walk<T, ED, POS, 256, LINED>;
+  constexpr int STRIDE = W::Staged::kStride;
+  constexpr int DB = (ED + 31) / 32;
+  constexpr int STEP = POS < 64 ? POS : 64;
+  constexpr int SUBS = STEP / 32;
+  extern __shared__ char shared[];
+  W w(p, shared);
+  const int h = (threadIdx.x & 63) >> 5;
+  const int key0 = (w.tile * 4 + w.wave) * 32;
+
+  typename M::Op k[ED / M::kDepth], v[ED / M::kDepth];
+  f32x16 dk[DB] = {}, dv[DB] = {};
+  if (w.begin < w.end) {
+    T* own = (T*)shared + w.wave * (Columns<T, ED>::kBytes / sizeof(T));
+    own_columns<T, ED>(k, own, (const T*)p.k + w.n * p.kn + w.hk * p.kh,
+                       p.ke, p.E, key0, w.total);
+    own_columns<T, ED>(v, own, (const T*)p.v + w.n * p.vn + w.hk * p.vh,
+                       p.ve, p.E, key0, w.total);
+    __syncthreads();
+    w.start();
+  }
+  for (int row = w.begin; row < w.end; row += POS) {
+    w.next(row);
+    if (key0 >= w.total) continue;  // no key of this wave's
+    const int i0 = row % p.pad;
+#pragma unroll 1
+    for (int col = 0; col < POS && i0 + col < p.Lq; col += STEP) {
+      f32x16 c[SUBS] = {}, dp[SUBS] = {};
+#pragma unroll
+      for (int b = 0; b < SUBS; ++b)
+#pragma unroll
+        for (int kk = 0; kk < ED / M::kDepth; ++kk) {
+          c[b] = M::mul(M::template first<STRIDE>(w.qt, kk, col + 32 * b),
+                        k[kk], c[b]);
+          dp[b] = M::mul(M::template first<STRIDE>(w.dt, kk, col + 32 * b),
+                         v[kk], dp[b]);
+        }
+      log_weights<T, SUBS, LINED>(p, c, w.lses + col, w.line, w.before,
+                                  w.behind, key0,
+                                  p.bias.query_start + i0 + col);
+#pragma unroll
+      for (int b = 0; b < SUBS; ++b) {
+        float e[16], ds[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 dl =
+              *(const f32x4*)(w.deltas + col + 32 * b + M::seq(4 * g, h));
+#pragma unroll
+          for (int j = 4 * g; j < 4 * g + 4; ++j) {
+            e[j] = __builtin_amdgcn_exp2f(c[b][j]);
+            ds[j] = e[j] * (dp[b][j] - dl[j & 3]);
+          }
+        }
+        typename M::Right pr, dr;
+        M::right(pr, e);
+        M::right(dr, ds);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          dv[d] = M::mul(
+              M::template second<STRIDE, ED>(w.dt, 32 * d, col + 32 * b), pr,
+              dv[d]);
+          dk[d] = M::mul(
+              M::template second<STRIDE, ED>(w.qt, 32 * d, col + 32 * b), dr,
+              dk[d]);
+        }
+      }
+    }
+  }
+  const int key = key0 + (threadIdx.x & 31);
+  w.template store<DB>(dk, (T*)p.dk, 0, key, p.scale);
+  w.template store<DB>(dv, (T*)p.dv, 1, key, 1.0f);
+}
+
+// For deep heads a wave's k, v, dk and dv alone are 192 registers, and a SIMD
+// would hold one wave, with nothing to run beside its waits. So two waves
+// share 32 keys: one has k and makes p and dv, the other has v and makes dp,
+// ds and dk. p goes from the one to the other through LDS in fp32, each lane
+// to its like, and the one's exponentials run beside the other's products.
+template <typename T, int ED, int POS, bool LINED>
+__global__ __launch_bounds__(512, 2) void attend_dkv_pair_kernel(Args p) {
+  using M = Mma<T>;
+  using W = Walk<T, ED, POS, 512, LINED>;
+  constexpr int STRIDE = W::Staged::kStride;
+  constexpr int DB = (ED + 31) / 32;
+  constexpr int SUBS = POS / 32;
+  static_assert(POS <= 64, "one step a tile");
+  extern __shared__ char shared[];
+  W w(p, shared);
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const bool second = w.wave >= 4;  // the wave with v
+  const int pair = w.wave & 3;
+  const int key0 = (w.tile * 4 + pair) * 32;
+  // (4 pairs, SUBS, 4, 64 lanes) of 4 floats
+  f32x4* hand = (f32x4*)(shared + 4 * W::Staged::kBytes + 16 * POS +
+                         (LINED ? (line_floats(p.bias.max_distance, true) + 3)
+                                          / 4 * 16
+                                : 0)) +
+                pair * SUBS * 256 + lane;
+
+  typename M::Op own[ED / M::kDepth];
+  f32x16 acc[DB] = {};
+  if (w.begin < w.end) {
+    const T* base = second ? (const T*)p.v + w.n * p.vn + w.hk * p.vh
+                           : (const T*)p.k + w.n * p.kn + w.hk * p.kh;
+    own_columns<T, ED>(
+        own, (T*)shared + w.wave * (Columns<T, ED>::kBytes / sizeof(T)),
+        base, second ? p.ve : p.ke, p.E, key0, w.total);
+    __syncthreads();
+    w.start();
+  }
+  for (int row = w.begin; row < w.end; row += POS) {
+    w.next(row);
+    const int i0 = row % p.pad;
+    const bool busy = key0 < w.total;
+    f32x16 c[SUBS] = {};
+    if (busy) {
+      const T* tile = second ? w.dt : w.qt;
+#pragma unroll
+      for (int b = 0; b < SUBS; ++b)
+#pragma unroll
+        for (int kk = 0; kk < ED / M::kDepth; ++kk)
+          c[b] = M::mul(M::template first<STRIDE>(tile, kk, 32 * b), own[kk],
+                        c[b]);
+      if (!second) {
+        log_weights<T, SUBS, LINED>(p, c, w.lses, w.line, w.before, w.behind,
+                                    key0, p.bias.query_start + i0);
+#pragma unroll
+        for (int b = 0; b < SUBS; ++b)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            f32x4 e;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              c[b][4 * g + j] = e[j] =
+                  __builtin_amdgcn_exp2f(c[b][4 * g + j]);
+            hand[(b * 4 + g) * 64] = e;
+          }
+      }
+    }
+    __syncthreads();
+    if (!busy) continue;
+    const T* tile = second ? w.qt : w.dt;
+#pragma unroll
+    for (int b = 0; b < SUBS; ++b) {
+      float s[16];
+      if (second) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 e = hand[(b * 4 + g) * 64];
+          const f32x4 dl =
+              *(const f32x4*)(w.deltas + 32 * b + M::seq(4 * g, h));
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            s[4 * g + j] = e[j] * (c[b][4 * g + j] - dl[j]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = c[b][j];
+      }
+      typename M::Right r;
+      M::right(r, s);
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+        acc[d] = M::mul(M::template second<STRIDE, ED>(tile, 32 * d, 32 * b),
+                        r, acc[d]);
+    }
+  }
+  const int key = key0 + (lane & 31);
+  w.template store<DB>(acc, second ? (T*)p.dk : (T*)p.dv, second ? 0 : 1, key,
+                       second ? p.scale : 1.0f);
 }
 
 // out[i] = sum of `splits` runs of `count`
@@ -460,9 +671,10 @@ std::vector<at::Tensor> cross_attention_bwd(
   const long pairs = (long)p.N * p.Hkv;
 
   p.out = dq.data_ptr();
-  p.pad = round_up(p.Lq, 32);
+  // with a bias, a workgroup's rows are one head's
+  p.pad = round_up(p.Lq, p.bias.table ? 128 : 32);
   p.tiles = sa::ceil_div((long)p.G * p.pad, 128);
-  p.splits = cut(dtable ? 1L << 40 : pairs * p.tiles, p.Lk, 64, &p.per_split);
+  p.splits = cut(dtable ? 1L << 40 : pairs * p.tiles, p.Lk, 128, &p.per_split);
   at::Tensor part, sums;
   if (p.splits > 1) {
     part = at::empty({p.splits, q.numel()}, f32);
@@ -480,13 +692,13 @@ std::vector<at::Tensor> cross_attention_bwd(
       constexpr int POS = tile_positions<T, ED>();
       const long blocks = pairs * p.splits * p.tiles;
       if (dtable)
-        launch(attend_dq_kernel<T, ED, 4, POS, true, true>, blocks, 256,
-               backward_lds<T, ED>(12 * line), p, stream);
+        launch(attend_dq_kernel<T, ED, POS, true, true>, blocks, 256,
+               backward_lds<T, ED>(9 * line), p, stream);
       else if (p.bias.table)
-        launch(attend_dq_kernel<T, ED, 4, POS, true, false>, blocks, 256,
-               backward_lds<T, ED>(4 * line), p, stream);
+        launch(attend_dq_kernel<T, ED, POS, true, false>, blocks, 256,
+               backward_lds<T, ED>(line), p, stream);
       else
-        launch(attend_dq_kernel<T, ED, 4, POS, false, false>, blocks, 256,
+        launch(attend_dq_kernel<T, ED, POS, false, false>, blocks, 256,
                backward_lds<T, ED>(0), p, stream);
     });
     if (p.splits > 1) {
@@ -531,12 +743,25 @@ std::vector<at::Tensor> cross_attention_bwd(
         p.part = part.data_ptr<float>();
       }
       const long blocks = pairs * p.splits * p.tiles;
-      if (p.bias.table)
-        launch(attend_dkv_kernel<T, ED, 4, POS, true>, blocks, 256,
-               backward_lds<T, ED>(8 * POS + line), p, stream);
-      else
-        launch(attend_dkv_kernel<T, ED, 4, POS, false>, blocks, 256,
-               backward_lds<T, ED>(8 * POS), p, stream);
+      const size_t lines =
+          p.bias.table ? line_floats(p.bias.max_distance, true) : 0;
+      if constexpr (ED * sizeof(T) > 128) {
+        const size_t lds = deep_lds<T, ED>(lines);
+        if (p.bias.table)
+          launch(attend_dkv_pair_kernel<T, ED, POS, true>, blocks, 512, lds,
+                 p, stream);
+        else
+          launch(attend_dkv_pair_kernel<T, ED, POS, false>, blocks, 512, lds,
+                 p, stream);
+      } else {
+        const size_t lds = backward_lds<T, ED>(16 * POS + 4 * lines);
+        if (p.bias.table)
+          launch(attend_dkv_kernel<T, ED, POS, true>, blocks, 256, lds, p,
+                 stream);
+        else
+          launch(attend_dkv_kernel<T, ED, POS, false>, blocks, 256, lds, p,
+                 stream);
+      }
     });
     if (p.splits > 1) {
       const int grid = sa::ceil_div(k.numel(), 256);
