@@ -171,28 +171,17 @@ void adam_step_packed(const at::Tensor& meta, const at::Tensor& sample,
                       double eps, double wd, double bc1, double bc2,
                       bool adamw);
 
-std::vector<at::Tensor> cross_attention_fwd(
-    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-    const c10::optional<at::Tensor>& lengths,
-    const c10::optional<at::Tensor>& table, double scale, long key_step,
-    long query_start, long max_distance, std::vector<long> thresholds,
-    bool stats);
-std::vector<at::Tensor> cross_attention_bwd(
-    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-    const c10::optional<at::Tensor>& lengths,
-    const c10::optional<at::Tensor>& table, const at::Tensor& out,
-    const at::Tensor& lse, const at::Tensor& dout, double scale,
-    long key_step, long query_start, long max_distance,
-    std::vector<long> thresholds, bool kv, bool dtable);
-std::vector<at::Tensor> gated_scan_fwd(
+at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k,
+                           const at::Tensor& v,
+                           const c10::optional<at::Tensor>& lengths,
+                           const c10::optional<at::Tensor>& table,
+                           c10::optional<double> scale, long key_step,
+                           long query_start, long max_distance,
+                           std::vector<long> thresholds);
+std::vector<at::Tensor> gated_scan_run(
     const at::Tensor& x, const at::Tensor& gate,
     const c10::optional<at::Tensor>& state,
-    const c10::optional<at::Tensor>& lengths, bool reverse, bool marked);
-std::vector<at::Tensor> gated_scan_bwd(
-    const at::Tensor& x, const at::Tensor& gate,
-    const c10::optional<at::Tensor>& lengths, const at::Tensor& marks,
-    const c10::optional<at::Tensor>& dh,
-    const c10::optional<at::Tensor>& dstate, bool reverse);
+    const c10::optional<at::Tensor>& lengths, bool reverse);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("pw_conv_fwd", &pw_conv_fwd, "pointwise conv forward (MFMA GEMM)");
@@ -272,12 +261,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "backward mask-scale for droppath_dropout_add");
   m.def("row_scale", &row_scale, "z = mask[n]*scale*y");
   m.def("adam_step_packed", &adam_step_packed, "fused adam step");
-  m.def("cross_attention_fwd", &cross_attention_fwd,
-        "attention to keys of another length (forward)");
-  m.def("cross_attention_bwd", &cross_attention_bwd,
-        "attention to keys of another length (backward)");
-  m.def("gated_scan_fwd", &gated_scan_fwd,
-        "gated linear recurrence (forward)");
-  m.def("gated_scan_bwd", &gated_scan_bwd,
-        "gated linear recurrence (backward)");
+  m.def("cross_attention", &cross_attention,
+        "attention to keys of another length, differentiable");
+  m.def("gated_scan", &gated_scan_run,
+        "gated linear recurrence, differentiable");
 }

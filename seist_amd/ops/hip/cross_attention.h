@@ -412,96 +412,46 @@ inline int cut(long blocks, long length, int step, int* per_split) {
   return sa::ceil_div(length, *per_split);
 }
 
-struct Inputs {
-  const at::Tensor &q, &k, &v;
-  const c10::optional<at::Tensor>&lengths, &table;
+// A call's tensors, as checked by checked(): unit stride along positions.
+struct Call {
+  at::Tensor q, k, v, table, lengths;  // the last two may be undefined
+  double scale;
+  long key_step, query_start, max_distance;
+  std::vector<long> thresholds;
 };
 
-inline Args args_of(const Inputs& in, double scale, long key_step, long query_start,
-             long max_distance, const std::vector<long>& thresholds) {
-  const auto &q = in.q, &k = in.k, &v = in.v;
-  TORCH_CHECK(q.is_cuda() && k.device() == q.device() &&
-                  v.device() == q.device(),
-              "cross_attention: q, k and v on one GPU required");
-  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes() &&
-                  k.size(0) == q.size(0) && k.size(2) == q.size(2),
-              "cross_attention: q (N, H, E, Lq), k and v (N, Hkv, E, Lk) "
-              "required");
-  TORCH_CHECK((q.scalar_type() == at::kBFloat16 ||
-               q.scalar_type() == at::kFloat) &&
-                  k.scalar_type() == q.scalar_type() &&
-                  v.scalar_type() == q.scalar_type(),
-              "cross_attention: q, k and v all bf16 or all fp32 required");
-  TORCH_CHECK(q.stride(3) == 1 && k.stride(3) == 1 && v.stride(3) == 1,
-              "cross_attention: unit stride along the positions required");
-  TORCH_CHECK(k.size(1) >= 1 && q.size(1) % k.size(1) == 0,
-              "cross_attention: H a multiple of Hkv required");
-  TORCH_CHECK(q.size(2) >= 1 && q.size(2) <= 128,
-              "cross_attention: E from 1 to 128 required");
-  TORCH_CHECK(q.size(3) < (1L << 28) && k.size(3) < (1L << 28) &&
-                  q.size(1) / k.size(1) * (q.size(3) + 128) < (1L << 30),
-              "cross_attention: sequences too long");
+inline Args args_of(const Call& c) {
   Args p = {};
-  p.q = q.data_ptr();
-  p.k = k.data_ptr();
-  p.v = v.data_ptr();
-  p.qn = q.stride(0), p.qh = q.stride(1), p.qe = q.stride(2);
-  p.kn = k.stride(0), p.kh = k.stride(1), p.ke = k.stride(2);
-  p.vn = v.stride(0), p.vh = v.stride(1), p.ve = v.stride(2);
-  p.N = q.size(0), p.H = q.size(1), p.Hkv = k.size(1), p.G = p.H / p.Hkv;
-  p.E = q.size(2), p.Lq = q.size(3), p.Lk = k.size(3);
-  p.scale = (float)scale;
-  const long size = q.element_size();
-  for (const auto* t : {&q, &k, &v})
-    TORCH_CHECK(t->stride(2) >= 0 &&
-                    (t->stride(2) * (p.E - 1) + t->size(3)) * size <
-                        (1L << 32),
-                "cross_attention: a head's channels have to lie within "
-                "4 GiB");
-  if (in.lengths.has_value()) {
-    const auto& l = *in.lengths;
-    TORCH_CHECK(l.device() == q.device() && l.scalar_type() == at::kInt &&
-                    l.is_contiguous() && l.dim() == 1 && l.size(0) == p.N,
-                "cross_attention: contiguous int32 kv_lengths (N) required");
-    p.lengths = l.data_ptr<int>();
-  }
-  if (in.table.has_value()) {
-    const auto& t = *in.table;
-    TORCH_CHECK(t.device() == q.device() && t.is_contiguous() &&
-                    t.dim() == 2 && t.size(0) == p.H &&
-                    t.scalar_type() == q.scalar_type(),
-                "cross_attention: contiguous bias table (H, buckets) of q's "
-                "type required");
+  p.q = c.q.data_ptr();
+  p.k = c.k.data_ptr();
+  p.v = c.v.data_ptr();
+  p.qn = c.q.stride(0), p.qh = c.q.stride(1), p.qe = c.q.stride(2);
+  p.kn = c.k.stride(0), p.kh = c.k.stride(1), p.ke = c.k.stride(2);
+  p.vn = c.v.stride(0), p.vh = c.v.stride(1), p.ve = c.v.stride(2);
+  p.N = c.q.size(0), p.H = c.q.size(1), p.Hkv = c.k.size(1);
+  p.G = p.H / p.Hkv;
+  p.E = c.q.size(2), p.Lq = c.q.size(3), p.Lk = c.k.size(3);
+  p.scale = (float)c.scale;
+  if (c.lengths.defined()) p.lengths = c.lengths.data_ptr<int>();
+  if (c.table.defined()) {
     Bias& b = p.bias;
-    b.table = t.data_ptr();
-    b.buckets = t.size(1);
+    b.table = c.table.data_ptr();
+    b.buckets = c.table.size(1);
     b.exact = b.buckets / 4;
-    b.steps = thresholds.size();
-    TORCH_CHECK(t.size(1) % 2 == 0 && b.buckets >= 4 &&
-                    b.buckets <= kMaxBuckets &&
-                    b.steps == b.buckets / 2 - b.exact - 1 &&
-                    b.steps <= kMaxThresholds,
-                "cross_attention: an even number of buckets from 4 to 64 "
-                "required");
-    TORCH_CHECK(max_distance > b.exact && max_distance <= kMaxDistance,
-                "cross_attention: max_distance over buckets/4 and at most ",
-                kMaxDistance, " required");
-    const long limit = 1L << 30;
-    TORCH_CHECK(key_step >= 1 && key_step < limit &&
-                    (double)key_step * (p.Lk + 128) < (double)limit &&
-                    std::abs(query_start) + p.Lq < limit,
-                "cross_attention: positions out of range");
-    b.max_distance = max_distance;
-    b.key_step = key_step;
-    b.query_start = query_start;
-    long least = b.exact;
-    for (int m = 0; m < b.steps; ++m) {
-      TORCH_CHECK(thresholds[m] >= least && thresholds[m] <= max_distance,
-                  "cross_attention: bucket thresholds out of order");
-      least = b.threshold[m] = thresholds[m];
-    }
+    b.steps = c.thresholds.size();
+    b.max_distance = c.max_distance;
+    b.key_step = c.key_step;
+    b.query_start = c.query_start;
+    for (int m = 0; m < b.steps; ++m) b.threshold[m] = c.thresholds[m];
   }
   return p;
 }
+
+// {out, lse}; lse is empty unless `stats`
+std::vector<at::Tensor> forward(const Call& c, bool stats);
+// {dq, dk, dv, dtable}; dk and dv empty unless `kv`, dtable unless `table`
+std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
+                                 const at::Tensor& lse,
+                                 const at::Tensor& dout, bool kv, bool table);
 
 }  // namespace attend

@@ -507,23 +507,13 @@ void launch_attend(const Args& p, long blocks, hipStream_t stream) {
   launch(attend_kernel<T, ED, QB, POS, false>, blocks, 256, lds, p, stream);
 }
 
-}  // namespace attend
-
-using namespace attend;
-
-// {out, lse}; lse is empty unless `stats`
-std::vector<at::Tensor> cross_attention_fwd(
-    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-    const c10::optional<at::Tensor>& lengths,
-    const c10::optional<at::Tensor>& table, double scale, long key_step,
-    long query_start, long max_distance, std::vector<long> thresholds,
-    bool stats) {
-  Args p = args_of({q, k, v, lengths, table}, scale, key_step, query_start,
-                   max_distance, thresholds);
-  const c10::DeviceGuard guard(q.device());
-  const auto f32 = q.options().dtype(at::kFloat);
-  auto out = at::empty(q.sizes(), q.options());
-  auto lse = at::empty({stats ? p.N : 0, p.H, p.Lq}, f32);
+std::vector<at::Tensor> forward(const Call& c, bool stats) {
+  Args p = args_of(c);
+  const c10::DeviceGuard guard(c.q.device());
+  const auto f32 = c.q.options().dtype(at::kFloat);
+  auto out = at::empty(c.q.sizes(), c.q.options());
+  at::Tensor lse;
+  if (stats) lse = at::empty({p.N, p.H, p.Lq}, f32);
   if (out.numel() == 0) return {out, lse};
   const auto stream = at::hip::getCurrentHIPStream().stream();
   p.out = out.data_ptr();
@@ -533,7 +523,7 @@ std::vector<at::Tensor> cross_attention_fwd(
   // two blocks of columns a wave where that still leaves every compute unit
   // two workgroups and a SIMD two waves (heads up to 64); fp32 matrix
   // products are too slow to wait for LDS
-  const bool twice = q.scalar_type() == at::kBFloat16 && p.E <= 64 && !p.bias.table &&
+  const bool twice = c.q.scalar_type() == at::kBFloat16 && p.E <= 64 && !p.bias.table &&
                      pairs * (p.G * (long)p.Lq / 256) >= 512;
   const int columns = twice ? 64 : 32;
   // with a bias, a workgroup's rows are one head's
@@ -541,15 +531,15 @@ std::vector<at::Tensor> cross_attention_fwd(
   const long rows = (long)p.G * p.pad;
   p.tiles = few ? 1 : sa::ceil_div(rows, 4 * columns);
   p.splits = cut(pairs * p.tiles, std::max(p.Lk, 1), 128, &p.per_split);
-  at::Tensor part, stat;
+  at::Tensor part;
   if (p.splits > 1) {
-    part = at::empty({p.splits * pairs * p.E * rows}, f32);
-    stat = at::empty({p.splits * pairs * 2 * rows}, f32);
+    const long sums = p.splits * pairs * p.E * rows;
+    part = at::empty({sums + p.splits * pairs * 2 * rows}, f32);
     p.part = part.data_ptr<float>();
-    p.stat = stat.data_ptr<float>();
+    p.stat = p.part + sums;
   }
   const long blocks = pairs * p.splits * p.tiles;
-  with_type(q.scalar_type(), [&](auto zero) {
+  with_type(c.q.scalar_type(), [&](auto zero) {
     using T = decltype(zero);
     with_depth(p.E, [&](auto depth) {
       constexpr int ED = decltype(depth)::value;
@@ -575,4 +565,170 @@ std::vector<at::Tensor> cross_attention_fwd(
              stream);
   });
   return {out, lse};
+}
+
+namespace {
+
+at::Tensor along_positions(const at::Tensor& t) {
+  return t.stride(3) == 1 ? t : t.contiguous();
+}
+
+std::string shape_of(const at::Tensor& t) {
+  return c10::str(t.sizes(), " ", t.scalar_type(), " on ", t.device());
+}
+
+// What the kernels take for granted. Lengths outside 0..Lk are held to it by
+// the kernels.
+Call checked(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+             const c10::optional<at::Tensor>& lengths,
+             const c10::optional<at::Tensor>& table,
+             c10::optional<double> scale, long key_step, long query_start,
+             long max_distance, std::vector<long> thresholds) {
+  TORCH_CHECK_VALUE(
+      q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes() &&
+          k.size(0) == q.size(0) && k.size(2) == q.size(2),
+      "cross_attention: q (N, H, E, Lq) and k, v (N, Hkv, E, Lk) are needed, "
+      "got ", shape_of(q), ", ", shape_of(k), ", ", shape_of(v));
+  const auto type = q.scalar_type();
+  TORCH_CHECK_VALUE(
+      (type == at::kBFloat16 || type == at::kFloat) &&
+          k.scalar_type() == type && v.scalar_type() == type,
+      "cross_attention: q, k and v have to be all float32 or all bfloat16, "
+      "got ", type, ", ", k.scalar_type(), ", ", v.scalar_type());
+  TORCH_CHECK_VALUE(q.is_cuda() && k.device() == q.device() &&
+                        v.device() == q.device(),
+                    "cross_attention: q, k and v have to be on one device");
+  const long H = q.size(1), Hkv = k.size(1), E = q.size(2), Lq = q.size(3),
+             Lk = k.size(3);
+  TORCH_CHECK_VALUE(Hkv > 0 && H % Hkv == 0, "cross_attention: ", H,
+                    " query heads cannot share ", Hkv, " key heads");
+  TORCH_CHECK_VALUE(E >= 1 && E <= 128, "cross_attention: heads of 1 to 128 "
+                    "channels are needed, got ", E);
+  TORCH_CHECK_VALUE(Lq < (1L << 28) && Lk < (1L << 28) &&
+                        H / Hkv * (Lq + 256) < (1L << 30),
+                    "cross_attention: sequences too long, ", shape_of(q), ", ",
+                    shape_of(k));
+  Call c = {along_positions(q), along_positions(k), along_positions(v), {},
+            {}, scale.value_or(1.0 / std::sqrt((double)E)), key_step,
+            query_start, max_distance, std::move(thresholds)};
+  TORCH_CHECK_VALUE(c.scale > 0 && std::isfinite((float)c.scale * kLog2e),
+                    "cross_attention: scale has to be positive, got ",
+                    c.scale);
+  for (const auto* t : {&c.q, &c.k, &c.v})
+    TORCH_CHECK_VALUE(
+        t->stride(2) >= 0 && (t->stride(2) * (E - 1) + t->size(3)) *
+                                     (long)t->element_size() < (1L << 32),
+        "cross_attention: a head's channels have to lie within 4 GiB");
+  if (lengths.has_value()) {
+    const auto& l = *lengths;
+    TORCH_CHECK_VALUE(
+        l.dim() == 1 && l.size(0) == q.size(0) &&
+            (l.scalar_type() == at::kInt || l.scalar_type() == at::kLong) &&
+            l.device() == q.device(),
+        "cross_attention: kv_lengths has to be [", q.size(0),
+        "] int32 or int64 on ", q.device(), ", got ", shape_of(l));
+    c.lengths = l.scalar_type() == at::kInt
+                    ? l.contiguous()
+                    : l.clamp(0, Lk).to(at::kInt).contiguous();
+  }
+  if (table.has_value()) {
+    const auto& t = *table;
+    TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == H &&
+                          t.scalar_type() == type && t.device() == q.device(),
+                      "cross_attention: bias_table has to be [", H,
+                      ", buckets] ", type, " on ", q.device(), ", got ",
+                      shape_of(t));
+    const long buckets = t.size(1), exact = buckets / 4;
+    TORCH_CHECK_VALUE(buckets % 2 == 0 && buckets >= 4 &&
+                          buckets <= kMaxBuckets &&
+                          (long)c.thresholds.size() ==
+                              buckets / 2 - exact - 1,
+                      "cross_attention: an even number of buckets from 4 to ",
+                      kMaxBuckets, " is needed, got ", buckets);
+    TORCH_CHECK_VALUE(max_distance > exact && max_distance <= kMaxDistance,
+                      "cross_attention: max_distance has to be over ", exact,
+                      " and at most ", kMaxDistance, ", got ", max_distance);
+    long least = exact;
+    for (const long m : c.thresholds) {
+      TORCH_CHECK_VALUE(m >= least && m <= max_distance,
+                        "cross_attention: bucket thresholds out of order");
+      least = m;
+    }
+    TORCH_CHECK_VALUE(key_step >= 1, "cross_attention: key_step has to be 1 "
+                      "or more, got ", key_step);
+    const long limit = 1L << 30;
+    TORCH_CHECK_VALUE(key_step < limit && key_step * (Lk + 128) < limit &&
+                          query_start > -limit && query_start < limit &&
+                          std::abs(query_start) + Lq + 256 < limit,
+                      "cross_attention: positions have to stay under 2**30");
+    c.table = t.contiguous();
+  }
+  return c;
+}
+
+// The node keeps the output and one logarithm a query; the backward pass
+// makes the scores again.
+class CrossAttention : public torch::autograd::Function<CrossAttention> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx,
+                            const at::Tensor& q, const at::Tensor& k,
+                            const at::Tensor& v,
+                            const c10::optional<at::Tensor>& table,
+                            const Call& call) {
+    auto r = attend::forward(call, true);
+    ctx->save_for_backward(
+        {q, k, v, call.table, call.lengths, r[0], r[1]});
+    ctx->saved_data["scale"] = call.scale;
+    ctx->saved_data["where"] = std::vector<int64_t>{
+        call.key_step, call.query_start, call.max_distance};
+    ctx->saved_data["thresholds"] = std::vector<int64_t>(
+        call.thresholds.begin(), call.thresholds.end());
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "cross_attention: second derivatives are not available");
+    const auto s = ctx->get_saved_variables();
+    const auto where = ctx->saved_data["where"].toIntVector();
+    const auto steps = ctx->saved_data["thresholds"].toIntVector();
+    const Call call = {s[0], s[1], s[2], s[3], s[4],
+                       ctx->saved_data["scale"].toDouble(), where[0],
+                       where[1], where[2],
+                       std::vector<long>(steps.begin(), steps.end())};
+    at::Tensor dout = along_positions(grads[0]);
+    if (dout.stride(2) < 0 ||
+        (dout.stride(2) * (dout.size(2) - 1) + dout.size(3)) *
+                (long)dout.element_size() >= (1L << 32))
+      dout = dout.contiguous();
+    const bool kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    const bool table = call.table.defined() && ctx->needs_input_grad(3);
+    auto r = attend::backward(call, s[5], s[6], dout, kv, table);
+    return {r[0], r[1], r[2], r[3], at::Tensor()};
+  }
+};
+
+}  // namespace
+}  // namespace attend
+
+at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k,
+                           const at::Tensor& v,
+                           const c10::optional<at::Tensor>& lengths,
+                           const c10::optional<at::Tensor>& table,
+                           c10::optional<double> scale, long key_step,
+                           long query_start, long max_distance,
+                           std::vector<long> thresholds) {
+  const auto call =
+      attend::checked(q, k, v, lengths, table, scale, key_step, query_start,
+                      max_distance, std::move(thresholds));
+  if (at::GradMode::is_enabled() &&
+      (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
+       (table.has_value() && table->requires_grad())))
+    return attend::CrossAttention::apply(
+        call.q, call.k, call.v,
+        call.table.defined() ? c10::optional<at::Tensor>(call.table)
+                             : c10::nullopt,
+        call);
+  return attend::forward(call, false)[0];
 }

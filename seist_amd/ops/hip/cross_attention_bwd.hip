@@ -623,44 +623,25 @@ __global__ __launch_bounds__(256) void sum_table_kernel(const float* in,
         (T)((sums[0][b] + sums[1][b]) + (sums[2][b] + sums[3][b]));
 }
 
-}  // namespace attend
-
-using namespace attend;
-
-// {dq, dk, dv, dtable}; dk and dv empty unless `kv`, dtable unless `dtable`
-std::vector<at::Tensor> cross_attention_bwd(
-    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-    const c10::optional<at::Tensor>& lengths,
-    const c10::optional<at::Tensor>& table, const at::Tensor& out,
-    const at::Tensor& lse, const at::Tensor& dout, double scale,
-    long key_step, long query_start, long max_distance,
-    std::vector<long> thresholds, bool kv, bool dtable) {
-  Args p = args_of({q, k, v, lengths, table}, scale, key_step, query_start,
-                   max_distance, thresholds);
-  TORCH_CHECK(dout.sizes() == q.sizes() && dout.stride(3) == 1 &&
-                  dout.stride(2) >= 0 &&
-                  (dout.stride(2) * (p.E - 1) + p.Lq) *
-                          (long)q.element_size() < (1L << 32) &&
-                  dout.scalar_type() == q.scalar_type() &&
-                  dout.device() == q.device(),
-              "cross_attention: dout like q required");
-  TORCH_CHECK(out.sizes() == q.sizes() && out.is_contiguous() &&
-                  out.scalar_type() == q.scalar_type() &&
-                  out.device() == q.device() && lse.is_contiguous() &&
-                  lse.numel() == (long)p.N * p.H * p.Lq &&
-                  lse.scalar_type() == at::kFloat &&
-                  lse.device() == q.device(),
-              "cross_attention: the forward pass's results required");
-  TORCH_CHECK(!dtable || p.bias.table, "cross_attention: no table given");
-  const c10::DeviceGuard guard(q.device());
-  const auto f32 = q.options().dtype(at::kFloat);
-  auto dq = at::empty(q.sizes(), q.options());
-  auto dk = at::empty(kv ? k.sizes() : at::IntArrayRef({0}), q.options());
-  auto dv = at::empty(kv ? v.sizes() : at::IntArrayRef({0}), q.options());
-  auto dt = at::empty(
-      dtable ? table->sizes() : at::IntArrayRef({0}), q.options());
-  if (q.numel() == 0 || k.numel() == 0)
-    return {dq.zero_(), dk.zero_(), dv.zero_(), dt.zero_()};
+std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
+                                 const at::Tensor& lse,
+                                 const at::Tensor& dout, bool kv,
+                                 bool table) {
+  Args p = args_of(c);
+  const c10::DeviceGuard guard(c.q.device());
+  const auto f32 = c.q.options().dtype(at::kFloat);
+  auto dq = at::empty(c.q.sizes(), c.q.options());
+  at::Tensor dk, dv, dt;
+  if (kv) {
+    dk = at::empty(c.k.sizes(), c.q.options());
+    dv = at::empty(c.k.sizes(), c.q.options());
+  }
+  if (table) dt = at::empty(c.table.sizes(), c.q.options());
+  if (c.q.numel() == 0 || c.k.numel() == 0) {
+    for (auto* t : {&dq, &dk, &dv, &dt})
+      if (t->defined()) t->zero_();
+    return {dq, dk, dv, dt};
+  }
   const auto stream = at::hip::getCurrentHIPStream().stream();
   auto delta = at::empty({p.N, p.H, p.Lq}, f32);
   p.o = out.data_ptr();
@@ -674,24 +655,24 @@ std::vector<at::Tensor> cross_attention_bwd(
   // with a bias, a workgroup's rows are one head's
   p.pad = round_up(p.Lq, p.bias.table ? 128 : 32);
   p.tiles = sa::ceil_div((long)p.G * p.pad, 128);
-  p.splits = cut(dtable ? 1L << 40 : pairs * p.tiles, p.Lk, 128, &p.per_split);
+  p.splits = cut(table ? 1L << 40 : pairs * p.tiles, p.Lk, 128, &p.per_split);
   at::Tensor part, sums;
   if (p.splits > 1) {
-    part = at::empty({p.splits, q.numel()}, f32);
+    part = at::empty({p.splits, c.q.numel()}, f32);
     p.part = part.data_ptr<float>();
   }
-  if (dtable) {
+  if (table) {
     sums = at::empty({p.N, p.H, p.pad / 32, p.bias.buckets}, f32);
     p.dbias = sums.data_ptr<float>();
   }
   const size_t line = (2 * p.bias.max_distance + 1) * 4;
-  with_type(q.scalar_type(), [&](auto zero) {
+  with_type(c.q.scalar_type(), [&](auto zero) {
     using T = decltype(zero);
     with_depth(p.E, [&](auto depth) {
       constexpr int ED = decltype(depth)::value;
       constexpr int POS = tile_positions<T, ED>();
       const long blocks = pairs * p.splits * p.tiles;
-      if (dtable)
+      if (table)
         launch(attend_dq_kernel<T, ED, POS, true, true>, blocks, 256,
                backward_lds<T, ED>(9 * line), p, stream);
       else if (p.bias.table)
@@ -702,11 +683,11 @@ std::vector<at::Tensor> cross_attention_bwd(
                backward_lds<T, ED>(0), p, stream);
     });
     if (p.splits > 1) {
-      sum_splits_kernel<T><<<sa::ceil_div(q.numel(), 256), 256, 0, stream>>>(
-          p.part, (T*)dq.data_ptr(), q.numel(), p.splits);
+      sum_splits_kernel<T><<<sa::ceil_div(c.q.numel(), 256), 256, 0, stream>>>(
+          p.part, (T*)dq.data_ptr(), c.q.numel(), p.splits);
       SA_CHECK_HIP(hipGetLastError());
     }
-    if (dtable) {
+    if (table) {
       const long rows = (long)p.N * (p.pad / 32);
       const int pieces = (int)std::min<long>((rows + 63) / 64, 256);
       const dim3 grid(p.H, pieces);
@@ -731,7 +712,7 @@ std::vector<at::Tensor> cross_attention_bwd(
   p.dk = dk.data_ptr();
   p.dv = dv.data_ptr();
   p.tiles = sa::ceil_div(p.Lk, 128);
-  with_type(q.scalar_type(), [&](auto zero) {
+  with_type(c.q.scalar_type(), [&](auto zero) {
     using T = decltype(zero);
     with_depth(p.E, [&](auto depth) {
       constexpr int ED = decltype(depth)::value;
@@ -739,7 +720,7 @@ std::vector<at::Tensor> cross_attention_bwd(
       p.pad = round_up(p.Lq, POS);
       p.splits = cut(pairs * p.tiles, (long)p.G * p.pad, POS, &p.per_split);
       if (p.splits > 1) {
-        part = at::empty({2, p.splits, k.numel()}, f32);
+        part = at::empty({2, p.splits, c.k.numel()}, f32);
         p.part = part.data_ptr<float>();
       }
       const long blocks = pairs * p.splits * p.tiles;
@@ -764,14 +745,16 @@ std::vector<at::Tensor> cross_attention_bwd(
       }
     });
     if (p.splits > 1) {
-      const int grid = sa::ceil_div(k.numel(), 256);
+      const int grid = sa::ceil_div(c.k.numel(), 256);
       sum_splits_kernel<T><<<grid, 256, 0, stream>>>(
-          p.part, (T*)dk.data_ptr(), k.numel(), p.splits);
+          p.part, (T*)dk.data_ptr(), c.k.numel(), p.splits);
       sum_splits_kernel<T><<<grid, 256, 0, stream>>>(
-          p.part + p.splits * k.numel(), (T*)dv.data_ptr(), k.numel(),
+          p.part + p.splits * c.k.numel(), (T*)dv.data_ptr(), c.k.numel(),
           p.splits);
       SA_CHECK_HIP(hipGetLastError());
     }
   });
   return {dq, dk, dv, dt};
 }
+
+}  // namespace attend

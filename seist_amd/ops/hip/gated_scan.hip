@@ -30,6 +30,7 @@
 
 #include "sa_common.h"
 
+namespace gated_scan {
 namespace {
 
 constexpr int kItems = 8;  // samples a lane holds
@@ -470,131 +471,192 @@ void launch(Which which, at::ScalarType type, bool rev, const ScanArgs& p,
   }
 }
 
-void check_pair(const at::Tensor& x, const at::Tensor& gate) {
-  TORCH_CHECK(x.is_cuda() && gate.device() == x.device(),
-              "gated_scan: x and gate on one GPU required");
-  TORCH_CHECK(x.dim() == 3 && gate.sizes() == x.sizes(),
-              "gated_scan: x and gate of one shape (N, C, L) required");
-  TORCH_CHECK((x.scalar_type() == at::kBFloat16 ||
-               x.scalar_type() == at::kFloat) &&
-                  gate.scalar_type() == x.scalar_type(),
-              "gated_scan: x and gate both bf16 or both fp32 required");
-  TORCH_CHECK(x.stride(2) == 1 && gate.stride(2) == 1,
-              "gated_scan: unit stride along L required");
-  TORCH_CHECK(x.size(2) >= 1 && x.size(2) < (1L << 30),
-              "gated_scan: L from 1 to 2^30 required");
-  TORCH_CHECK(x.size(0) * x.size(1) < (1L << 31) / 64,
-              "gated_scan: too many rows");
-}
+// A call's tensors, as checked by checked(): x and gate with unit stride
+// along L, the rest contiguous; state and lengths may be undefined.
+struct Call {
+  at::Tensor x, gate, state, lengths;
+  bool reverse;
+};
 
-void check_state(const c10::optional<at::Tensor>& s, const at::Tensor& x) {
-  if (!s.has_value()) return;
-  TORCH_CHECK(s->device() == x.device() && s->scalar_type() == at::kFloat &&
-                  s->is_contiguous() && s->dim() == 2 &&
-                  s->size(0) == x.size(0) && s->size(1) == x.size(1),
-              "gated_scan: contiguous fp32 state (N, C) required");
-}
-
-ScanArgs args_of(const at::Tensor& x, const at::Tensor& gate,
-                 const c10::optional<at::Tensor>& lengths, const Deal& deal) {
+ScanArgs args_of(const Call& c, const Deal& deal) {
   ScanArgs p = {};
-  p.x = x.data_ptr();
-  p.gate = gate.data_ptr();
-  if (lengths.has_value()) {
-    TORCH_CHECK(lengths->device() == x.device() &&
-                    lengths->scalar_type() == at::kInt &&
-                    lengths->is_contiguous() && lengths->dim() == 1 &&
-                    lengths->size(0) == x.size(0),
-                "gated_scan: contiguous int32 lengths (N) required");
-    p.lengths = lengths->data_ptr<int>();
-  }
-  p.xn = x.stride(0);
-  p.xc = x.stride(1);
-  p.gn = gate.stride(0);
-  p.gc = gate.stride(1);
-  p.rows = x.size(0) * x.size(1);
-  p.C = x.size(1);
-  p.L = x.size(2);
+  p.x = c.x.data_ptr();
+  p.gate = c.gate.data_ptr();
+  if (c.lengths.defined()) p.lengths = c.lengths.data_ptr<int>();
+  p.xn = c.x.stride(0);
+  p.xc = c.x.stride(1);
+  p.gn = c.gate.stride(0);
+  p.gc = c.gate.stride(1);
+  p.rows = c.x.size(0) * c.x.size(1);
+  p.C = c.x.size(1);
+  p.L = c.x.size(2);
   p.chunks = deal.chunks;
   p.segments = deal.segments;
   p.per_segment = deal.per_segment;
   return p;
 }
 
-}  // namespace
-
-// {h, last state, marks}; marks is empty unless `marked`
-std::vector<at::Tensor> gated_scan_fwd(
-    const at::Tensor& x, const at::Tensor& gate,
-    const c10::optional<at::Tensor>& state,
-    const c10::optional<at::Tensor>& lengths, bool reverse, bool marked) {
-  check_pair(x, gate);
-  check_state(state, x);
-  const c10::DeviceGuard guard(x.device());
-  const auto f32 = x.options().dtype(at::kFloat);
-  auto h = at::empty(x.sizes(), x.options());
-  auto last = at::empty({x.size(0), x.size(1)}, f32);
+// {h, last state, marks}; marks only if `marked`
+std::vector<at::Tensor> forward(const Call& c, bool marked) {
+  const c10::DeviceGuard guard(c.x.device());
+  const auto f32 = c.x.options().dtype(at::kFloat);
+  auto h = at::empty(c.x.sizes(), c.x.options());
+  auto last = at::empty({c.x.size(0), c.x.size(1)}, f32);
   const long rows = last.numel();
-  const Deal deal(rows, x.size(2));
-  auto marks = at::empty({marked ? rows : 0, deal.chunks}, f32);
+  at::Tensor marks, maps;
   if (rows == 0) return {h, last, marks};
-  ScanArgs p = args_of(x, gate, lengths, deal);
-  p.state = state.has_value() ? state->data_ptr<float>() : nullptr;
-  p.marks = marked ? marks.data_ptr<float>() : nullptr;
+  const Deal deal(rows, c.x.size(2));
+  ScanArgs p = args_of(c, deal);
+  if (marked) {
+    marks = at::empty({rows, deal.chunks}, f32);
+    p.marks = marks.data_ptr<float>();
+  }
+  if (c.state.defined()) p.state = c.state.data_ptr<float>();
   p.out = h.data_ptr();
   p.last = last.data_ptr<float>();
   const auto stream = at::hip::getCurrentHIPStream().stream();
-  at::Tensor maps;
+  const auto type = c.x.scalar_type();
   if (deal.segments > 1) {
     maps = at::empty({rows, deal.segments, 2}, f32);
     p.maps = p.maps_out = maps.data_ptr<float>();
-    launch(MAP, x.scalar_type(), reverse, p, deal, stream);
+    launch(MAP, type, c.reverse, p, deal, stream);
   }
-  launch(SCAN, x.scalar_type(), reverse, p, deal, stream);
+  launch(SCAN, type, c.reverse, p, deal, stream);
   return {h, last, marks};
 }
 
-// {dx, dgate, d(first state)}
-std::vector<at::Tensor> gated_scan_bwd(
-    const at::Tensor& x, const at::Tensor& gate,
-    const c10::optional<at::Tensor>& lengths, const at::Tensor& marks,
-    const c10::optional<at::Tensor>& dh,
-    const c10::optional<at::Tensor>& dstate, bool reverse) {
-  check_pair(x, gate);
-  check_state(dstate, x);
-  const c10::DeviceGuard guard(x.device());
-  const auto f32 = x.options().dtype(at::kFloat);
-  auto dx = at::empty(x.sizes(), x.options());
-  auto dgate = at::empty(x.sizes(), x.options());
-  auto first = at::empty({x.size(0), x.size(1)}, f32);
+// {dx, dgate, d(first state)} of dh and d(last state), each maybe undefined
+std::vector<at::Tensor> backward(const Call& c, const at::Tensor& marks,
+                                 const at::Tensor& dh,
+                                 const at::Tensor& dstate) {
+  const c10::DeviceGuard guard(c.x.device());
+  const auto f32 = c.x.options().dtype(at::kFloat);
+  auto dx = at::empty(c.x.sizes(), c.x.options());
+  auto dgate = at::empty(c.x.sizes(), c.x.options());
+  auto first = at::empty({c.x.size(0), c.x.size(1)}, f32);
   const long rows = first.numel();
   if (rows == 0) return {dx, dgate, first};
-  const Deal deal(rows, x.size(2));
-  TORCH_CHECK(marks.device() == x.device() &&
-                  marks.scalar_type() == at::kFloat &&
-                  marks.is_contiguous() && marks.dim() == 2 &&
-                  marks.size(0) == rows && marks.size(1) == deal.chunks,
-              "gated_scan: the forward pass's marks required");
-  ScanArgs p = args_of(x, gate, lengths, deal);
-  if (dh.has_value()) {
-    TORCH_CHECK(dh->device() == x.device() && dh->sizes() == x.sizes() &&
-                    dh->scalar_type() == x.scalar_type() &&
-                    dh->is_contiguous(),
-                "gated_scan: contiguous dh like x required");
-    p.dh = dh->data_ptr();
-  }
-  p.dstate = dstate.has_value() ? dstate->data_ptr<float>() : nullptr;
+  const Deal deal(rows, c.x.size(2));
+  ScanArgs p = args_of(c, deal);
+  if (dh.defined()) p.dh = dh.data_ptr();
+  if (dstate.defined()) p.dstate = dstate.data_ptr<float>();
   p.marks = marks.data_ptr<float>();
   p.out = dx.data_ptr();
   p.out2 = dgate.data_ptr();
   p.last = first.data_ptr<float>();
   const auto stream = at::hip::getCurrentHIPStream().stream();
+  const auto type = c.x.scalar_type();
   at::Tensor maps;
   if (deal.segments > 1) {
     maps = at::empty({rows, deal.segments, 2}, f32);
     p.maps = p.maps_out = maps.data_ptr<float>();
-    launch(MAP_BACK, x.scalar_type(), reverse, p, deal, stream);
+    launch(MAP_BACK, type, c.reverse, p, deal, stream);
   }
-  launch(SCAN_BACK, x.scalar_type(), reverse, p, deal, stream);
+  launch(SCAN_BACK, type, c.reverse, p, deal, stream);
   return {dx, dgate, first};
+}
+
+std::string shape_of(const at::Tensor& t) {
+  return c10::str(t.sizes(), " ", t.scalar_type(), " on ", t.device());
+}
+
+at::Tensor along_samples(const at::Tensor& t) {
+  return t.stride(2) == 1 ? t : t.contiguous();
+}
+
+// What the kernels take for granted. Lengths outside 0..L are held to it by
+// the kernels.
+Call checked(const at::Tensor& x, const at::Tensor& gate,
+             const c10::optional<at::Tensor>& state,
+             const c10::optional<at::Tensor>& lengths, bool reverse) {
+  TORCH_CHECK_VALUE(
+      x.dim() == 3 && gate.sizes() == x.sizes() && x.size(2) >= 1,
+      "gated_scan: x and gate of one shape (N, C, L), L at least 1, are "
+      "needed, got ", shape_of(x), " and ", shape_of(gate));
+  const auto type = x.scalar_type();
+  TORCH_CHECK_VALUE(
+      (type == at::kBFloat16 || type == at::kFloat) &&
+          gate.scalar_type() == type,
+      "gated_scan: x and gate have to be both float32 or both bfloat16, got ",
+      type, " and ", gate.scalar_type());
+  TORCH_CHECK_VALUE(x.is_cuda() && gate.device() == x.device(),
+                    "gated_scan: x and gate have to be on one device");
+  TORCH_CHECK_VALUE(x.size(2) < (1L << 30) &&
+                        x.size(0) * x.size(1) < (1L << 24),
+                    "gated_scan: under 2**30 samples and 2**24 rows are "
+                    "needed, got ", shape_of(x));
+  Call c = {along_samples(x), along_samples(gate), {}, {}, reverse};
+  if (state.has_value()) {
+    TORCH_CHECK_VALUE(
+        state->sizes() == x.sizes().slice(0, 2) &&
+            state->scalar_type() == at::kFloat &&
+            state->device() == x.device(),
+        "gated_scan: state has to be ", x.sizes().slice(0, 2),
+        " float32 on ", x.device(), ", got ", shape_of(*state));
+    c.state = state->contiguous();
+  }
+  if (lengths.has_value()) {
+    const auto& l = *lengths;
+    TORCH_CHECK_VALUE(
+        l.dim() == 1 && l.size(0) == x.size(0) &&
+            (l.scalar_type() == at::kInt || l.scalar_type() == at::kLong) &&
+            l.device() == x.device(),
+        "gated_scan: lengths has to be [", x.size(0),
+        "] int32 or int64 on ", x.device(), ", got ", shape_of(l));
+    c.lengths = l.scalar_type() == at::kInt
+                    ? l.contiguous()
+                    : l.clamp(0, x.size(2)).to(at::kInt).contiguous();
+  }
+  return c;
+}
+
+// The node keeps the inputs and the fp32 state at each chunk's start.
+class GatedScan : public torch::autograd::Function<GatedScan> {
+ public:
+  static torch::autograd::variable_list forward(
+      torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+      const at::Tensor& gate, const c10::optional<at::Tensor>& state,
+      const Call& call) {
+    auto r = gated_scan::forward(call, true);
+    ctx->save_for_backward({x, gate, call.lengths, r[2]});
+    ctx->saved_data["reverse"] = call.reverse;
+    ctx->saved_data["state"] = state.has_value();
+    ctx->set_materialize_grads(false);
+    return {r[0], r[1]};
+  }
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "gated_scan: second derivatives are not available");
+    const auto s = ctx->get_saved_variables();
+    const Call call = {s[0], s[1], {}, s[2],
+                       ctx->saved_data["reverse"].toBool()};
+    for (auto& g : grads)
+      if (g.defined()) g = g.contiguous();
+    auto r = gated_scan::backward(call, s[3], grads[0], grads[1]);
+    const bool state = ctx->saved_data["state"].toBool();
+    return {r[0], r[1], state ? r[2] : at::Tensor(), at::Tensor()};
+  }
+};
+
+}  // namespace
+}  // namespace gated_scan
+
+// {h, last state}
+std::vector<at::Tensor> gated_scan_run(
+    const at::Tensor& x, const at::Tensor& gate,
+    const c10::optional<at::Tensor>& state,
+    const c10::optional<at::Tensor>& lengths, bool reverse) {
+  const auto call = gated_scan::checked(x, gate, state, lengths, reverse);
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || gate.requires_grad() ||
+       (state.has_value() && state->requires_grad())))
+    return gated_scan::GatedScan::apply(
+        call.x, call.gate,
+        call.state.defined() ? c10::optional<at::Tensor>(call.state)
+                             : c10::nullopt,
+        call);
+  auto r = gated_scan::forward(call, false);
+  return {r[0], r[1]};
 }

@@ -29,23 +29,13 @@ def _refuse(op: str, what: str):
 
 
 def _check_lengths(op: str, name: str, lengths, like: torch.Tensor):
-    if lengths is None:
-        return None
-    if lengths.dim() != 1 or lengths.size(0) != like.size(0) \
-            or lengths.dtype not in (torch.int32, torch.int64) \
-            or lengths.device != like.device:
+    if lengths is not None and (
+            lengths.dim() != 1 or lengths.size(0) != like.size(0)
+            or lengths.dtype not in (torch.int32, torch.int64)
+            or lengths.device != like.device):
         _refuse(op, f"{name} has to be ({like.size(0)},) int32 or int64 on "
                     f"{like.device}, got {tuple(lengths.shape)} "
                     f"{lengths.dtype} on {lengths.device}")
-    if lengths.dtype != torch.int32:
-        # a length past the end counts as the whole, one under zero as none
-        lengths = lengths.clamp(0, 2 ** 31 - 1).to(torch.int32)
-    return lengths.contiguous()
-
-
-def _rows_of_samples(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with unit stride along its last axis; other strides stay."""
-    return t if t.stride(-1) == 1 else t.contiguous()
 
 
 # ---------------------------------------------------------------------------
@@ -107,30 +97,40 @@ def relative_position_buckets(distance: torch.Tensor, num_buckets: int,
 # ---------------------------------------------------------------------------
 
 
-class _CrossAttention(torch.autograd.Function):
-    """Saves the output and one logarithm a query; scores are made again in
-    the backward pass (a per-query kernel for dq and the bias, a per-key
-    kernel for dk and dv)."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, table, lengths, conf):
-        out, lse = ext().cross_attention_fwd(q, k, v, lengths, table, *conf,
-                                             True)
-        ctx.save_for_backward(q, k, v, table, lengths, out, lse)
-        ctx.conf = conf
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        q, k, v, table, lengths, out, lse = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dq, dk, dv, dtable = ext().cross_attention_bwd(
-            q, k, v, lengths, table, out, lse, _rows_of_samples(dout),
-            *ctx.conf, need[1] or need[2], need[3])
-        return (dq if need[0] else None, dk if need[1] else None,
-                dv if need[2] else None, dtable if need[3] else None, None,
-                None)
+def _check_cross_attention(q, k, v, kv_lengths, bias_table, scale, key_step,
+                           query_start):
+    op = "cross_attention"
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape \
+            or k.size(0) != q.size(0) or k.size(2) != q.size(2):
+        _refuse(op, "q (N, H, E, Lq) and k, v (N, Hkv, E, Lk) are needed, "
+                    f"got {tuple(q.shape)}, {tuple(k.shape)}, "
+                    f"{tuple(v.shape)}")
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        _refuse(op, "q, k and v have to be all float32 or all bfloat16, got "
+                    f"{q.dtype}, {k.dtype}, {v.dtype}")
+    if k.device != q.device or v.device != q.device:
+        _refuse(op, "q, k and v have to be on one device")
+    H, E = q.size(1), q.size(2)
+    if k.size(1) == 0 or H % k.size(1):
+        _refuse(op, f"{H} query heads cannot share {k.size(1)} key heads")
+    if not 1 <= E <= _MAX_DEPTH:
+        _refuse(op, f"heads of 1 to {_MAX_DEPTH} channels are needed, got "
+                    f"{E}")
+    if scale is not None and not 0 < scale < math.inf:
+        _refuse(op, f"scale has to be positive, got {scale}")
+    _check_lengths(op, "kv_lengths", kv_lengths, q)
+    if bias_table is not None:
+        if bias_table.dim() != 2 or bias_table.size(0) != H \
+                or bias_table.dtype != q.dtype \
+                or bias_table.device != q.device:
+            _refuse(op, f"bias_table has to be ({H}, buckets) {q.dtype} on "
+                        f"{q.device}, got {tuple(bias_table.shape)} "
+                        f"{bias_table.dtype} on {bias_table.device}")
+        if key_step < 1:
+            _refuse(op, f"key_step has to be 1 or more, got {key_step}")
+        if key_step * (k.size(3) + 128) >= 2 ** 30 \
+                or abs(query_start) + q.size(3) + 256 >= 2 ** 30:
+            _refuse(op, "positions have to stay under 2**30")
 
 
 def _cross_attention_plain(q, k, v, lengths, table, scale, key_step,
@@ -186,54 +186,20 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
     A query with no key left gives zeros and no gradient.
     """
-    op = "cross_attention"
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape \
-            or k.size(0) != q.size(0) or k.size(2) != q.size(2):
-        _refuse(op, "q (N, H, E, Lq) and k, v (N, Hkv, E, Lk) are needed, "
-                    f"got {tuple(q.shape)}, {tuple(k.shape)}, "
-                    f"{tuple(v.shape)}")
-    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
-        _refuse(op, "q, k and v have to be all float32 or all bfloat16, got "
-                    f"{q.dtype}, {k.dtype}, {v.dtype}")
-    if k.device != q.device or v.device != q.device:
-        _refuse(op, "q, k and v have to be on one device")
-    H, E = q.size(1), q.size(2)
-    if k.size(1) == 0 or H % k.size(1):
-        _refuse(op, f"{H} query heads cannot share {k.size(1)} key heads")
-    if not 1 <= E <= _MAX_DEPTH:
-        _refuse(op, f"heads of 1 to {_MAX_DEPTH} channels are needed, got "
-                    f"{E}")
-    lengths = _check_lengths(op, "kv_lengths", kv_lengths, q)
     thresholds = []
-    if bias_table is not None:
-        if bias_table.dim() != 2 or bias_table.size(0) != H \
-                or bias_table.dtype != q.dtype \
-                or bias_table.device != q.device:
-            _refuse(op, f"bias_table has to be ({H}, buckets) {q.dtype} on "
-                        f"{q.device}, got {tuple(bias_table.shape)} "
-                        f"{bias_table.dtype} on {bias_table.device}")
-        _check_buckets(op, bias_table.size(1), max_distance)
-        if key_step < 1:
-            _refuse(op, f"key_step has to be 1 or more, got {key_step}")
-        if key_step * (k.size(3) + 128) >= 2 ** 30 \
-                or abs(query_start) + q.size(3) >= 2 ** 30:
-            _refuse(op, "positions have to stay under 2**30")
+    if bias_table is not None and bias_table.dim() == 2:
+        _check_buckets("cross_attention", bias_table.size(1), max_distance)
         thresholds = _bucket_thresholds(bias_table.size(1), max_distance)
+    if use_native(q):  # with its own checks, the same as those below
+        return ext().cross_attention(q, k, v, kv_lengths, bias_table, scale,
+                                     key_step, query_start, max_distance,
+                                     thresholds)
+    _check_cross_attention(q, k, v, kv_lengths, bias_table, scale, key_step,
+                           query_start)
     if scale is None:
-        scale = 1.0 / math.sqrt(E)
-    if not use_native(q):
-        return _cross_attention_plain(q, k, v, lengths, bias_table, scale,
-                                      key_step, query_start, max_distance)
-    q, k, v = _rows_of_samples(q), _rows_of_samples(k), _rows_of_samples(v)
-    if bias_table is not None:
-        bias_table = bias_table.contiguous()
-    conf = (scale, key_step, query_start, max_distance, thresholds)
-    if torch.is_grad_enabled() and (
-            q.requires_grad or k.requires_grad or v.requires_grad
-            or (bias_table is not None and bias_table.requires_grad)):
-        return _CrossAttention.apply(q, k, v, bias_table, lengths, conf)
-    return ext().cross_attention_fwd(q, k, v, lengths, bias_table, *conf,
-                                     False)[0]
+        scale = 1.0 / math.sqrt(q.size(2))
+    return _cross_attention_plain(q, k, v, kv_lengths, bias_table, scale,
+                                  key_step, query_start, max_distance)
 
 
 # ---------------------------------------------------------------------------
@@ -241,30 +207,23 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 # ---------------------------------------------------------------------------
 
 
-class _GatedScan(torch.autograd.Function):
-    """Saves the inputs and the fp32 state at the start of each chunk; the
-    backward pass makes the states in between again instead of reading h."""
-
-    @staticmethod
-    def forward(ctx, x, gate, state, lengths, reverse):
-        h, last, marks = ext().gated_scan_fwd(x, gate, state, lengths,
-                                              reverse, True)
-        ctx.save_for_backward(x, gate, lengths, marks)
-        ctx.reverse = reverse
-        ctx.set_materialize_grads(False)
-        return h, last
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dh, dlast):
-        x, gate, lengths, marks = ctx.saved_tensors
-        dx, dgate, dstate = ext().gated_scan_bwd(
-            x, gate, lengths, marks,
-            None if dh is None else dh.contiguous(),
-            None if dlast is None else dlast.contiguous(), ctx.reverse)
-        need = ctx.needs_input_grad
-        return (dx if need[0] else None, dgate if need[1] else None,
-                dstate if need[2] else None, None, None)
+def _check_gated_scan(x, gate, state, lengths):
+    op = "gated_scan"
+    if x.dim() != 3 or gate.shape != x.shape or x.size(2) < 1:
+        _refuse(op, "x and gate of one shape (N, C, L), L at least 1, are "
+                    f"needed, got {tuple(x.shape)} and {tuple(gate.shape)}")
+    if x.dtype not in _DTYPES or gate.dtype != x.dtype:
+        _refuse(op, "x and gate have to be both float32 or both bfloat16, "
+                    f"got {x.dtype} and {gate.dtype}")
+    if gate.device != x.device:
+        _refuse(op, "x and gate have to be on one device")
+    if state is not None and (state.shape != x.shape[:2]
+                              or state.dtype != torch.float32
+                              or state.device != x.device):
+        _refuse(op, f"state has to be {tuple(x.shape[:2])} float32 on "
+                    f"{x.device}, got {tuple(state.shape)} {state.dtype} on "
+                    f"{state.device}")
+    _check_lengths(op, "lengths", lengths, x)
 
 
 def _gated_scan_plain(x, gate, state, lengths, reverse):
@@ -309,30 +268,8 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor,
     zero, the state stays, and nothing is read into the result. ``reverse``
     runs from the last sample that counts to the first.
     """
-    op = "gated_scan"
-    if x.dim() != 3 or gate.shape != x.shape or x.size(2) < 1:
-        _refuse(op, "x and gate of one shape (N, C, L), L at least 1, are "
-                    f"needed, got {tuple(x.shape)} and {tuple(gate.shape)}")
-    if x.dtype not in _DTYPES or gate.dtype != x.dtype:
-        _refuse(op, "x and gate have to be both float32 or both bfloat16, "
-                    f"got {x.dtype} and {gate.dtype}")
-    if gate.device != x.device:
-        _refuse(op, "x and gate have to be on one device")
-    if state is not None and (state.shape != x.shape[:2]
-                              or state.dtype != torch.float32
-                              or state.device != x.device):
-        _refuse(op, f"state has to be {tuple(x.shape[:2])} float32 on "
-                    f"{x.device}, got {tuple(state.shape)} {state.dtype} on "
-                    f"{state.device}")
-    lengths = _check_lengths(op, "lengths", lengths, x)
-    if not use_native(x):
-        return _gated_scan_plain(x, gate, state, lengths, reverse)
-    x, gate = _rows_of_samples(x), _rows_of_samples(gate)
-    if state is not None:
-        state = state.contiguous()
-    if torch.is_grad_enabled() and (
-            x.requires_grad or gate.requires_grad
-            or (state is not None and state.requires_grad)):
-        return _GatedScan.apply(x, gate, state, lengths, reverse)
-    h, last, _ = ext().gated_scan_fwd(x, gate, state, lengths, reverse, False)
-    return h, last
+    if use_native(x):  # with its own checks, the same as those below
+        h, last = ext().gated_scan(x, gate, state, lengths, reverse)
+        return h, last
+    _check_gated_scan(x, gate, state, lengths)
+    return _gated_scan_plain(x, gate, state, lengths, reverse)
