@@ -37,7 +37,7 @@ struct Args {
   float* delta;    // (N, H, Lq)
   float* part;     // split results, fp32
   float* stat;     // split maxima and sums
-  float* dbias;    // (N, Hkv*G, row tiles, buckets)
+  float* dbias;    // (N * splits, H, tiles of 128 rows, buckets)
   const int* lengths;
   long qn, qh, qe, kn, kh, ke, vn, vh, ve, dn, dh, de;
   int N, H, Hkv, G, E, Lq, Lk;

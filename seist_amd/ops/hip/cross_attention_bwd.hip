@@ -23,16 +23,26 @@ size_t deep_lds(size_t lines) {
   return std::max<size_t>(staged, 8 * Columns<T, ED>::kBytes);
 }
 
-// A wave's sums of ds by distance (one line for each half) and beyond the
-// last one, added up by bucket. `out` is the wave's first row's place.
-__device__ __forceinline__ void fold_table(const Args& p, const float* lines,
+// A workgroup's sums of ds by distance (a line for each of its 8 half waves)
+// and beyond the last one (a wave's in each lane), added up by bucket, each
+// in the same order every time. `ends`: 8 floats of LDS.
+__device__ __forceinline__ void fold_table(const Bias& b, const float* lines,
                                            float before, float behind,
-                                           float* out, bool live) {
-  const Bias& b = p.bias;
-  const int lane = threadIdx.x & 63, half = b.buckets / 2;
-  const int wide = 2 * b.max_distance + 1;
+                                           float* ends, float* out) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int half = b.buckets / 2, wide = 2 * b.max_distance + 1;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    before += __shfl_xor(before, off);
+    behind += __shfl_xor(behind, off);
+  }
+  if (lane == 0) {
+    ends[wave] = before;
+    ends[4 + wave] = behind;
+  }
+  __syncthreads();
 #pragma unroll 1
-  for (int at = 0; at < b.buckets; ++at) {
+  for (int at = wave; at < b.buckets; at += 4) {
     const bool after = at >= half;
     const int m = after ? at - half : at;
     int lo = m, hi = m + 1;
@@ -41,14 +51,15 @@ __device__ __forceinline__ void fold_table(const Args& p, const float* lines,
       hi = m == half - 1 ? b.max_distance : b.threshold[m - b.exact];
     }
     if (after && lo == 0) lo = 1;
-    float v = m < half - 1 ? 0.0f : after ? behind : before;
+    float v = m == half - 1 && lane < 4 ? ends[4 * after + lane] : 0.0f;
     for (int n = lo + lane; n < hi; n += 64) {
       const int d = b.max_distance + (after ? n : -n);
-      v += lines[d] + lines[wide + d];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v += lines[k * wide + d];
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-    if (live && lane == 0) out[at] = v;
+    if (lane == 0) out[at] = v;
   }
 }
 
@@ -112,7 +123,8 @@ void attend_dq_kernel(Args p) {
 
   float* line = (float*)(shared + 4 * Staged::kBytes) +
                 line_middle(far, false);
-  float* lines = line + far + 1;  // the wave's ds by distance, a line a half
+  // the wave's ds by distance, a line for each of its halves
+  float* lines = line + far + 1 + wave * 2 * (2 * far + 1);
   float before = 0.0f, behind = 0.0f;      // bias past the last bucket
   float ds_before = 0.0f, ds_behind = 0.0f;
   if (LINED) {  // the workgroup's rows are one head's
@@ -120,7 +132,6 @@ void attend_dq_kernel(Args p) {
     before = bias_of<T>(p.bias, head, -far);
     behind = bias_of<T>(p.bias, head, far);
     if (TABLE) {
-      lines += wave * 2 * (2 * far + 1);
       for (int d = lane; d < 2 * (2 * far + 1); d += 64) lines[d] = 0.0f;
     }
   }
@@ -233,13 +244,11 @@ void attend_dq_kernel(Args p) {
     if (TWICE && walk == 0) delta = both_sum(delta);
   }
   const int rows = p.G * p.pad;
-  if (TABLE) {
-    wave_fence();
-    fold_table(p, lines, ds_before, ds_behind,
-               p.dbias + (((long)n * p.H + head) * (p.pad / 32) + i0 / 32) *
-                             p.bias.buckets,
-               first < rows);
-  }
+  if (TABLE)  // a workgroup's rows are one head's, and there are some
+    fold_table(p.bias, line + far + 1, ds_before, ds_behind,
+               line + far + 1 + 8 * (2 * far + 1),
+               p.dbias + (((long)(n * p.splits + split) * p.H + head) *
+                              (p.pad / 128) + i0 / 128) * p.bias.buckets);
   if (first >= rows || !live) return;
   if (split == 0 && h == 0) p.delta[stat] = delta;
   const long to = ((long)n * p.H + head) * p.E * p.Lq + i;
@@ -612,10 +621,18 @@ __global__ __launch_bounds__(256) void sum_table_kernel(const float* in,
   const long each = (rows + gridDim.y - 1) / gridDim.y;
   const long begin = blockIdx.y * each, end = min(rows, begin + each);
   float v = 0.0f;
-  if (b < buckets)
-    for (long r = begin + lane; r < end; r += 4)
-      v += in[((r / tiles * H + blockIdx.x) * tiles + r % tiles) * buckets +
-              b];
+  // 8 rows at a time, so that their loads are on the way together
+  for (long r0 = begin + lane; r0 < end && b < buckets; r0 += 32) {
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const long r = min(r0 + 4 * i, end - 1);
+      w[i] = in[((r / tiles * H + blockIdx.x) * tiles + r % tiles) * buckets +
+                b];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += r0 + 4 * i < end ? w[i] : 0.0f;
+  }
   sums[lane][b] = v;
   __syncthreads();
   if (lane == 0 && b < buckets)
@@ -655,14 +672,17 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
   // with a bias, a workgroup's rows are one head's
   p.pad = round_up(p.Lq, p.bias.table ? 128 : 32);
   p.tiles = sa::ceil_div((long)p.G * p.pad, 128);
-  p.splits = cut(table ? 1L << 40 : pairs * p.tiles, p.Lk, 128, &p.per_split);
+  // no cut where delta comes from a first walk over all keys
+  const bool twice = table && c.q.scalar_type() == at::kBFloat16;
+  p.splits =
+      cut(twice ? 1L << 40 : pairs * p.tiles, p.Lk, 128, &p.per_split);
   at::Tensor part, sums;
   if (p.splits > 1) {
     part = at::empty({p.splits, c.q.numel()}, f32);
     p.part = part.data_ptr<float>();
   }
   if (table) {
-    sums = at::empty({p.N, p.H, p.pad / 32, p.bias.buckets}, f32);
+    sums = at::empty({p.N * p.splits, p.H, p.pad / 128, p.bias.buckets}, f32);
     p.dbias = sums.data_ptr<float>();
   }
   const size_t line = (2 * p.bias.max_distance + 1) * 4;
@@ -674,7 +694,7 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
       const long blocks = pairs * p.splits * p.tiles;
       if (table)
         launch(attend_dq_kernel<T, ED, POS, true, true>, blocks, 256,
-               backward_lds<T, ED>(9 * line), p, stream);
+               backward_lds<T, ED>(9 * line + 32), p, stream);
       else if (p.bias.table)
         launch(attend_dq_kernel<T, ED, POS, true, false>, blocks, 256,
                backward_lds<T, ED>(line), p, stream);
@@ -688,17 +708,17 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
       SA_CHECK_HIP(hipGetLastError());
     }
     if (table) {
-      const long rows = (long)p.N * (p.pad / 32);
-      const int pieces = (int)std::min<long>((rows + 63) / 64, 256);
+      const int of = p.N * p.splits, tiles = p.pad / 128;
+      const int pieces =
+          (int)std::min<long>(((long)of * tiles + 511) / 512, 256);
       const dim3 grid(p.H, pieces);
       if (pieces == 1) {
         sum_table_kernel<T><<<grid, 256, 0, stream>>>(
-            p.dbias, (T*)dt.data_ptr(), p.N, p.H, p.pad / 32,
-            p.bias.buckets);
+            p.dbias, (T*)dt.data_ptr(), of, p.H, tiles, p.bias.buckets);
       } else {
         auto some = at::empty({p.H, pieces, p.bias.buckets}, f32);
         sum_table_kernel<float><<<grid, 256, 0, stream>>>(
-            p.dbias, some.data_ptr<float>(), p.N, p.H, p.pad / 32,
+            p.dbias, some.data_ptr<float>(), of, p.H, tiles,
             p.bias.buckets);
         sum_table_kernel<T><<<dim3(p.H, 1), 256, 0, stream>>>(
             some.data_ptr<float>(), (T*)dt.data_ptr(), 1, p.H, pieces,

@@ -4,7 +4,7 @@
 //
 // A step is the map h -> A*h + B, and maps compose:
 // (A2, B2) after (A1, B1) is (A2*A1, A2*B1 + B2). A lane composes 8
-// neighbouring samples in registers, a row's lanes join their maps with
+// neighbouring samples (4 in fp32) in registers, a row's lanes join their maps with
 // log2 exchanges, waves join theirs through LDS, and the state carries from
 // chunk to chunk, so a sample is read once and written once. The gradient
 // runs the other way: with u_t = a_t * G_t, G_t = dh_t + u_{t+1},
@@ -33,7 +33,9 @@
 namespace gated_scan {
 namespace {
 
-constexpr int kItems = 8;  // samples a lane holds
+// samples a lane holds: 16 bytes, so that a wave reads 1 KB in one piece
+template <typename T>
+constexpr int kItems = 16 / sizeof(T);
 
 struct ScanArgs {
   const void* x;
@@ -70,103 +72,146 @@ __device__ __forceinline__ void gates(float g, float& a, float& keep) {
   const float hi = m * kHi;
   const float lo = fmaf(m, kLo, fmaf(m, kHi, -hi));
   float e = __builtin_amdgcn_exp2f(hi);
-  if (m > -100.0f) e = fmaf(e, lo * 0.693147180559945f, e);
-  const float r = 1.0f / (1.0f + e);
+  if (e > 0.0f) e = fmaf(e, lo * 0.693147180559945f, e);
+  const float r = __builtin_amdgcn_rcpf(1.0f + e);
   const float s = e * r;
   a = g < 0.0f ? s : r;
   keep = g < 0.0f ? r : s;
 }
 
-// 8 samples from p on; rows start anywhere, so the 16-byte accesses are not
-// aligned
+// a lane's 8 samples of scan index s0.., in the words that they fill in
+// memory, so that a load is not waited for before its samples are used; rows
+// start anywhere, so the 16-byte accesses are not aligned
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[kItems]) {
-  T t[kItems];
-  __builtin_memcpy(t, p, sizeof(t));
+struct Items {
+  static constexpr int kEach = 4 / sizeof(T);  // samples of a word
+  unsigned w[kItems<T> / kEach];
+  template <bool REV>
+  __device__ __forceinline__ void load(const T* row, int s0, int L,
+                                       bool whole) {
+    if (whole) {
+      __builtin_memcpy(w, row + (REV ? L - kItems<T> - s0 : s0), sizeof(w));
+    } else {
 #pragma unroll
-  for (int i = 0; i < kItems; ++i) v[i] = (float)t[i];
-}
-
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[kItems]) {
-  T t[kItems];
-#pragma unroll
-  for (int i = 0; i < kItems; ++i) t[i] = (T)v[i];
-  __builtin_memcpy(p, t, sizeof(t));
-}
-
-// v[i] = sample of scan index s0+i, 0 outside the row
-template <typename T, bool REV>
-__device__ __forceinline__ void load_items(const T* row, long s0, int L,
-                                           float (&v)[kItems]) {
-  if (s0 + kItems <= L) {
-    float t[kItems];
-    load8(row + (REV ? L - kItems - s0 : s0), t);
-#pragma unroll
-    for (int i = 0; i < kItems; ++i) v[i] = REV ? t[kItems - 1 - i] : t[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const long s = s0 + i;
-      v[i] = s < L ? (float)row[REV ? L - 1 - s : s] : 0.0f;
+      for (int k = 0; k < kItems<T>; ++k) {  // as they come in memory
+        const int s = min(s0 + (REV ? kItems<T> - 1 - k : k), L - 1);
+        unsigned v = 0;
+        __builtin_memcpy(&v, row + (REV ? L - 1 - s : s), sizeof(T));
+        if (k % kEach == 0) w[k / kEach] = v;
+        else w[k / kEach] |= v << 16;
+      }
     }
   }
-}
-
-template <typename T, bool REV>
-__device__ __forceinline__ void store_items(T* row, long s0, int L,
-                                            const float (&v)[kItems]) {
-  if (s0 + kItems <= L) {
-    float t[kItems];
+  template <bool REV>
+  __device__ __forceinline__ float at(int i) const {
+    const int k = REV ? kItems<T> - 1 - i : i;
+    const unsigned v = w[k / kEach];
+    if (kEach == 1) return __uint_as_float(v);
+    return __uint_as_float(k % kEach == 0 ? v << 16 : v & 0xffff0000u);
+  }
+  template <bool REV>
+  __device__ __forceinline__ void set(const float (&x)[kItems<T>]) {
+    T v[kItems<T>];
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) t[i] = REV ? v[kItems - 1 - i] : v[i];
-    store8(row + (REV ? L - kItems - s0 : s0), t);
-  } else {
+    for (int k = 0; k < kItems<T>; ++k) v[k] = (T)x[REV ? kItems<T> - 1 - k : k];
+    __builtin_memcpy(w, v, sizeof(w));
+  }
+  template <bool REV>
+  __device__ __forceinline__ void store(T* row, int s0, int L,
+                                        bool whole) const {
+    if (whole) {
+      __builtin_memcpy(row + (REV ? L - kItems<T> - s0 : s0), w, sizeof(w));
+    } else {
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const long s = s0 + i;
-      if (s < L) row[REV ? L - 1 - s : s] = (T)v[i];
+      for (int k = 0; k < kItems<T>; ++k) {
+        const int s = s0 + (REV ? kItems<T> - 1 - k : k);
+        const unsigned v = w[k / kEach] >> (k % kEach * 16);
+        if (s < L)
+          __builtin_memcpy(row + (REV ? L - 1 - s : s), &v, sizeof(T));
+      }
     }
   }
+};
+
+// one step of a scan over a wave's lanes: composes with the map CTRL away
+template <int CTRL, int ROWS>
+__device__ __forceinline__ Map dpp_after(Map m) {
+  const Map o = {
+      __int_as_float(__builtin_amdgcn_update_dpp(
+          __float_as_int(1.0f), __float_as_int(m.a), CTRL, ROWS, 0xf, false)),
+      __int_as_float(__builtin_amdgcn_update_dpp(
+          0, __float_as_int(m.b), CTRL, ROWS, 0xf, false))};
+  return after(m, o);
+}
+
+// each lane's map after those of the lanes below it, over 16 lanes or 64:
+// shifts by 1, 2, 4, 8 within 16 lanes, then the last of 16 lanes to the
+// next 16, then the last of 32 to the upper half
+template <int LANES>
+__device__ __forceinline__ Map scan_lanes(Map m) {
+  m = dpp_after<0x111, 0xf>(m);
+  m = dpp_after<0x112, 0xf>(m);
+  m = dpp_after<0x114, 0xf>(m);
+  m = dpp_after<0x118, 0xf>(m);
+  if (LANES == 64) {
+    m = dpp_after<0x142, 0xa>(m);
+    m = dpp_after<0x143, 0xc>(m);
+  }
+  return m;
+}
+
+__device__ __forceinline__ Map of_lane(Map m, int lane) {
+  return {__int_as_float(
+              __builtin_amdgcn_readlane(__float_as_int(m.a), lane)),
+          __int_as_float(
+              __builtin_amdgcn_readlane(__float_as_int(m.b), lane))};
 }
 
 // What stands before (UP) or behind (!UP) each lane of its row's lanes, and
 // the whole, all in scan order. A row has LPR lanes of one wave and W waves.
-template <int LPR, int W, bool UP>
 struct Joined {
   Map before, whole;
 };
 
 template <int LPR, int W, bool UP>
-__device__ __forceinline__ Joined<LPR, W, UP> join(Map m, Map* lds) {
-  const int lane = threadIdx.x & (LPR - 1);
-#pragma unroll
-  for (int d = 1; d < LPR; d <<= 1) {
-    Map o;
-    o.a = UP ? __shfl_up(m.a, d, LPR) : __shfl_down(m.a, d, LPR);
-    o.b = UP ? __shfl_up(m.b, d, LPR) : __shfl_down(m.b, d, LPR);
-    if (UP ? lane >= d : lane + d < LPR) m = after(m, o);
-  }
-  Joined<LPR, W, UP> j;
-  j.whole.a = __shfl(m.a, UP ? LPR - 1 : 0, LPR);
-  j.whole.b = __shfl(m.b, UP ? LPR - 1 : 0, LPR);
-  j.before.a = UP ? __shfl_up(m.a, 1, LPR) : __shfl_down(m.a, 1, LPR);
-  j.before.b = UP ? __shfl_up(m.b, 1, LPR) : __shfl_down(m.b, 1, LPR);
-  if (lane == (UP ? 0 : LPR - 1)) j.before = {1.0f, 0.0f};
-  if constexpr (W > 1) {
-    const int wave = threadIdx.x / sa::kWave;
-    if (lane == 0) lds[wave] = j.whole;
-    __syncthreads();
-    Map all = {1.0f, 0.0f};
-    Map head = all;
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const int w = UP ? i : W - 1 - i;
-      if (w == wave) head = all;
-      all = after(lds[w], all);
+__device__ __forceinline__ Joined join(Map m, Map* lds) {
+  Joined j;
+  if constexpr (LPR == 64) {
+    const int lane = threadIdx.x & 63;
+    if (!UP) m = {__shfl(m.a, 63 - lane), __shfl(m.b, 63 - lane)};
+    m = scan_lanes<64>(m);
+    j.whole = of_lane(m, 63);
+    j.before = {__shfl_up(m.a, 1), __shfl_up(m.b, 1)};
+    if (lane == 0) j.before = {1.0f, 0.0f};
+    if constexpr (W > 1) {
+      const int wave =
+          __builtin_amdgcn_readfirstlane(threadIdx.x / sa::kWave);
+      if (lane == 0) lds[UP ? wave : W - 1 - wave] = j.whole;
+      __syncthreads();
+      Map all = {1.0f, 0.0f};
+      if (lane < W) all = lds[lane];
+      all = scan_lanes<16>(all);
+      const int at = UP ? wave : W - 1 - wave;
+      if (at > 0) j.before = after(j.before, of_lane(all, at - 1));
+      j.whole = of_lane(all, W - 1);
     }
-    j.before = after(j.before, head);
-    j.whole = all;
+    if (!UP)
+      j.before = {__shfl(j.before.a, 63 - lane),
+                  __shfl(j.before.b, 63 - lane)};
+  } else {
+    const int lane = threadIdx.x & (LPR - 1);
+#pragma unroll
+    for (int d = 1; d < LPR; d <<= 1) {
+      Map o;
+      o.a = UP ? __shfl_up(m.a, d, LPR) : __shfl_down(m.a, d, LPR);
+      o.b = UP ? __shfl_up(m.b, d, LPR) : __shfl_down(m.b, d, LPR);
+      if (UP ? lane >= d : lane + d < LPR) m = after(m, o);
+    }
+    j.whole.a = __shfl(m.a, UP ? LPR - 1 : 0, LPR);
+    j.whole.b = __shfl(m.b, UP ? LPR - 1 : 0, LPR);
+    j.before.a = UP ? __shfl_up(m.a, 1, LPR) : __shfl_down(m.a, 1, LPR);
+    j.before.b = UP ? __shfl_up(m.b, 1, LPR) : __shfl_down(m.b, 1, LPR);
+    if (lane == (UP ? 0 : LPR - 1)) j.before = {1.0f, 0.0f};
   }
   return j;
 }
@@ -185,82 +230,146 @@ __device__ __forceinline__ float through(const float* maps, int segments,
       const int at = UP ? k : segments - 1 - k;
       m = {maps[2 * at], maps[2 * at + 1]};
     }
-#pragma unroll
-    for (int d = 1; d < sa::kWave; d <<= 1) {
-      Map o = {__shfl_up(m.a, d), __shfl_up(m.b, d)};
-      if (lane >= d) m = after(m, o);
-    }
-    state = fmaf(__shfl(m.a, sa::kWave - 1), state,
-                 __shfl(m.b, sa::kWave - 1));
+    m = of_lane(scan_lanes<64>(m), 63);
+    state = fmaf(m.a, state, m.b);
   }
   return state;
 }
 
-template <int LPR, int W>
+// A lane's place: its row, and the chunks of the row that it walks. Only
+// chunks that hold a valid sample are walked; first..begin and end..last
+// have none.
+template <typename T, int LPR, int W, bool REV>
 struct Place {
-  long row;
-  int lane, seg, first, end;  // the chunks of this row that are walked
+  static constexpr int kChunk = LPR * W * kItems<T>;
+  const ScanArgs& p;
+  long row, n, c;
+  int lane, seg, first, last, begin, end, len;
   bool live;
-  __device__ __forceinline__ Place(const ScanArgs& p) {
-    lane = threadIdx.x & (LPR * W - 1);
-    if (W > 1) lane = threadIdx.x;
+  __device__ __forceinline__ Place(const ScanArgs& args) : p(args) {
+    lane = W > 1 ? threadIdx.x : threadIdx.x & (LPR - 1);
     seg = blockIdx.y;
     row = W > 1 ? (long)blockIdx.x
                 : ((long)blockIdx.x * blockDim.x + threadIdx.x) / LPR;
+    if (LPR == 64 && W == 1)  // a wave's own, so that it stays scalar
+      row = __builtin_amdgcn_readfirstlane((int)row);
     live = row < p.rows;
     if (!live) row = p.rows - 1;  // reads in bounds, writes nothing
+    n = row / p.C;
+    c = row % p.C;
+    len = p.lengths == nullptr ? p.L : max(0, min(p.lengths[n], p.L));
     first = seg * p.per_segment;
-    end = min(first + p.per_segment, p.chunks);
+    last = min(first + p.per_segment, p.chunks);
+    begin = first;
+    end = last;
+    if (LPR == 64) {
+      const int from = REV ? (p.L - len) / kChunk : 0;
+      const int to = REV ? p.chunks : sa_ceil(len, kChunk);
+      begin = min(max(begin, from), last);
+      end = max(min(end, to), begin);
+      if (len == 0) end = begin;
+    }
+  }
+  __device__ static int sa_ceil(int a, int b) { return (a + b - 1) / b; }
+  __device__ __forceinline__ int start(int chunk) const {
+    return chunk * kChunk + lane * kItems<T>;  // under 2^30 + 2^13
+  }
+  // every sample of the chunk (of the row) in bounds; and valid
+  __device__ __forceinline__ bool whole(int chunk) const {
+    return (chunk + 1) * kChunk <= p.L;
+  }
+  __device__ __forceinline__ bool full(int chunk) const {
+    return whole(chunk) && (REV ? chunk * kChunk >= p.L - len
+                                : (chunk + 1) * kChunk <= len);
+  }
+  __device__ __forceinline__ bool valid(int s) const {
+    return s < p.L && (REV ? p.L - 1 - s : s) < len;
+  }
+  __device__ __forceinline__ const T* x() const {
+    return (const T*)p.x + n * p.xn + c * p.xc;
+  }
+  __device__ __forceinline__ const T* gate() const {
+    return (const T*)p.gate + n * p.gn + c * p.gc;
+  }
+  __device__ __forceinline__ const T* dh() const {
+    return p.dh ? (const T*)p.dh + row * p.L : nullptr;
+  }
+  // zeros where no sample is valid
+  __device__ __forceinline__ void blank(T* out) const {
+    if (!live) return;
+    Items<T> zero;
+#pragma unroll
+    for (unsigned& w : zero.w) w = 0;
+    for (int chunk = first; chunk < last; ++chunk)
+      if (chunk < begin || chunk >= end)
+        zero.template store<REV>(out, start(chunk), p.L, whole(chunk));
   }
 };
 
-__device__ __forceinline__ int valid_length(const ScanArgs& p, long n) {
-  if (p.lengths == nullptr) return p.L;
-  return max(0, min(p.lengths[n], p.L));
-}
-
-// a, keep and x of a lane's samples; outside the valid length a sample
-// passes the state on
-template <typename T, bool REV>
-__device__ __forceinline__ void take(const T* x, const T* gate, long s0,
-                                     int L, int len, float (&xs)[kItems],
-                                     float (&a)[kItems],
-                                     float (&keep)[kItems]) {
-  float g[kItems];
-  load_items<T, REV>(gate, s0, L, g);
-  if (x != nullptr) load_items<T, REV>(x, s0, L, xs);
+// a, keep and one more of a lane's samples; outside the valid length a
+// sample passes the state on
+template <bool REV, bool FULL, typename T, typename P>
+__device__ __forceinline__ void take(const P& at, int chunk,
+                                     const Items<T>& gate,
+                                     const Items<T>& more, bool given,
+                                     float (&a)[kItems<T>],
+                                     float (&keep)[kItems<T>],
+                                     float (&m)[kItems<T>]) {
 #pragma unroll
-  for (int i = 0; i < kItems; ++i) {
-    gates(g[i], a[i], keep[i]);
-    const long s = s0 + i;
-    const bool in = s < L && (REV ? L - 1 - s : s) < len;
-    if (!in) {
-      a[i] = 1.0f;
-      keep[i] = 0.0f;
-      xs[i] = 0.0f;
-    }
+  for (int i = 0; i < kItems<T>; ++i) {
+    gates(gate.template at<REV>(i), a[i], keep[i]);
+    m[i] = given ? more.template at<REV>(i) : 0.0f;
+  }
+  if (!FULL) {
+    const int s0 = at.start(chunk);
+#pragma unroll
+    for (int i = 0; i < kItems<T>; ++i)
+      if (!at.valid(s0 + i)) {
+        a[i] = 1.0f;
+        keep[i] = 0.0f;
+        m[i] = 0.0f;
+      }
   }
 }
 
-template <typename T, int LPR, int W, bool REV>
-__global__ __launch_bounds__(W > 1 ? W * 64 : 256) void scan_map_kernel(
-    ScanArgs p) {
+// Whether a chunk has only valid samples is the same for all of its lanes;
+// those chunks go without a comparison.
+template <typename P, typename F>
+__device__ __forceinline__ void for_chunk(const P& at, int chunk, F f) {
+  if (at.full(chunk)) f(std::true_type());
+  else f(std::false_type());
+}
+
+#define SCAN_KERNEL \
+  template <typename T, int LPR, int W, bool REV> \
+  __global__ __launch_bounds__(W > 1 ? W * 64 : 256) void
+
+// a segment's map
+SCAN_KERNEL scan_map_kernel(ScanArgs p) {
   __shared__ Map lds[2][W];
-  const Place<LPR, W> at(p);
-  const long n = at.row / p.C, c = at.row % p.C;
-  const int len = valid_length(p, n);
-  const T* x = (const T*)p.x + n * p.xn + c * p.xc;
-  const T* gate = (const T*)p.gate + n * p.gn + c * p.gc;
+  const Place<T, LPR, W, REV> at(p);
+  const T *x = at.x(), *gate = at.gate();
+  Items<T> xi, gi;
+  auto fetch = [&](int chunk) {
+    const bool whole = at.whole(chunk);
+    gi.template load<REV>(gate, at.start(chunk), p.L, whole);
+    xi.template load<REV>(x, at.start(chunk), p.L, whole);
+  };
+  if (at.begin < at.end) fetch(at.begin);
   Map m = {1.0f, 0.0f};
-  for (int chunk = at.first; chunk < at.end; ++chunk) {
-    const long s0 = ((long)chunk * LPR * W + at.lane) * kItems;
-    float xs[kItems], a[kItems], keep[kItems];
-    take<T, REV>(x, gate, s0, p.L, len, xs, a, keep);
-    Map own = {1.0f, 0.0f};
+  for (int chunk = at.begin; chunk < at.end; ++chunk) {
+    for_chunk(at, chunk, [&](auto is_full) {
+      constexpr bool FULL = decltype(is_full)::value;
+      float xs[kItems<T>], a[kItems<T>], keep[kItems<T>];
+      const Items<T> gn = gi, xn = xi;
+      if (chunk + 1 < at.end) fetch(chunk + 1);
+      take<REV, FULL>(at, chunk, gn, xn, true, a, keep, xs);
+      Map own = {1.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < kItems; ++i)
-      own = {own.a * a[i], fmaf(a[i], own.b, keep[i] * xs[i])};
-    m = after(join<LPR, W, true>(own, lds[chunk & 1]).whole, m);
+      for (int i = 0; i < kItems<T>; ++i)
+        own = {own.a * a[i], fmaf(a[i], own.b, keep[i] * xs[i])};
+      m = after(join<LPR, W, true>(own, lds[chunk & 1]).whole, m);
+    });
   }
   if (at.live && at.lane == 0) {
     float* o = p.maps_out + (at.row * p.segments + at.seg) * 2;
@@ -269,26 +378,32 @@ __global__ __launch_bounds__(W > 1 ? W * 64 : 256) void scan_map_kernel(
   }
 }
 
-// u_t = a_t * (dh_t + u_{t+1}) over a segment
-template <typename T, int LPR, int W, bool REV>
-__global__ __launch_bounds__(W > 1 ? W * 64 : 256) void scan_map_back_kernel(
-    ScanArgs p) {
+// the same for u_t = a_t * (dh_t + u_{t+1})
+SCAN_KERNEL scan_map_back_kernel(ScanArgs p) {
   __shared__ Map lds[2][W];
-  const Place<LPR, W> at(p);
-  const long n = at.row / p.C, c = at.row % p.C;
-  const int len = valid_length(p, n);
-  const T* gate = (const T*)p.gate + n * p.gn + c * p.gc;
-  const T* dh = p.dh ? (const T*)p.dh + at.row * p.L : nullptr;
+  const Place<T, LPR, W, REV> at(p);
+  const T *dh = at.dh(), *gate = at.gate();
+  Items<T> di, gi;
+  auto fetch = [&](int chunk) {
+    const bool whole = at.whole(chunk);
+    gi.template load<REV>(gate, at.start(chunk), p.L, whole);
+    if (dh) di.template load<REV>(dh, at.start(chunk), p.L, whole);
+  };
+  if (at.begin < at.end) fetch(at.end - 1);
   Map m = {1.0f, 0.0f};
-  for (int chunk = at.end - 1; chunk >= at.first; --chunk) {
-    const long s0 = ((long)chunk * LPR * W + at.lane) * kItems;
-    float d[kItems] = {}, a[kItems], keep[kItems];
-    take<T, REV>(dh, gate, s0, p.L, len, d, a, keep);
-    Map own = {1.0f, 0.0f};
+  for (int chunk = at.end - 1; chunk >= at.begin; --chunk) {
+    for_chunk(at, chunk, [&](auto is_full) {
+      constexpr bool FULL = decltype(is_full)::value;
+      float d[kItems<T>], a[kItems<T>], keep[kItems<T>];
+      const Items<T> gn = gi, dn = di;
+      if (chunk > at.begin) fetch(chunk - 1);
+      take<REV, FULL>(at, chunk, gn, dn, dh != nullptr, a, keep, d);
+      Map own = {1.0f, 0.0f};
 #pragma unroll
-    for (int i = kItems - 1; i >= 0; --i)
-      own = {own.a * a[i], a[i] * (d[i] + own.b)};
-    m = after(join<LPR, W, false>(own, lds[chunk & 1]).whole, m);
+      for (int i = kItems<T> - 1; i >= 0; --i)
+        own = {own.a * a[i], a[i] * (d[i] + own.b)};
+      m = after(join<LPR, W, false>(own, lds[chunk & 1]).whole, m);
+    });
   }
   if (at.live && at.lane == 0) {
     float* o = p.maps_out + (at.row * p.segments + at.seg) * 2;
@@ -297,126 +412,156 @@ __global__ __launch_bounds__(W > 1 ? W * 64 : 256) void scan_map_back_kernel(
   }
 }
 
-template <typename T, int LPR, int W, bool REV>
-__global__ __launch_bounds__(W > 1 ? W * 64 : 256) void scan_kernel(
-    ScanArgs p) {
+SCAN_KERNEL scan_kernel(ScanArgs p) {
   __shared__ Map lds[2][W];
-  const Place<LPR, W> at(p);
-  const long n = at.row / p.C, c = at.row % p.C;
-  const int len = valid_length(p, n);
-  const T* x = (const T*)p.x + n * p.xn + c * p.xc;
-  const T* gate = (const T*)p.gate + n * p.gn + c * p.gc;
+  const Place<T, LPR, W, REV> at(p);
+  const T *x = at.x(), *gate = at.gate();
   T* out = (T*)p.out + at.row * p.L;
+  Items<T> xi, gi;
+  auto fetch = [&](int chunk) {
+    const bool whole = at.whole(chunk);
+    gi.template load<REV>(gate, at.start(chunk), p.L, whole);
+    xi.template load<REV>(x, at.start(chunk), p.L, whole);
+  };
+  if (at.begin < at.end) fetch(at.begin);
   float state = p.state ? p.state[at.row] : 0.0f;
   if (p.segments > 1)
     state = through<true>(p.maps + at.row * p.segments * 2, p.segments,
                           at.seg, state);
-  for (int chunk = at.first; chunk < at.end; ++chunk) {
-    const long s0 = ((long)chunk * LPR * W + at.lane) * kItems;
-    if (p.marks && at.live && at.lane == 0)
-      p.marks[at.row * p.chunks + chunk] = state;
-    float xs[kItems], a[kItems], keep[kItems];
-    take<T, REV>(x, gate, s0, p.L, len, xs, a, keep);
-    Map own = {1.0f, 0.0f};
+  for (int chunk = at.begin; chunk < at.end; ++chunk) {
+    for_chunk(at, chunk, [&](auto is_full) {
+      constexpr bool FULL = decltype(is_full)::value;
+      if (p.marks && at.live && at.lane == 0)
+        p.marks[at.row * p.chunks + chunk] = state;
+      float xs[kItems<T>], a[kItems<T>], keep[kItems<T>];
+      const Items<T> gn = gi, xn = xi;
+      if (chunk + 1 < at.end) fetch(chunk + 1);
+      take<REV, FULL>(at, chunk, gn, xn, true, a, keep, xs);
+      Map own = {1.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < kItems; ++i)
-      own = {own.a * a[i], fmaf(a[i], own.b, keep[i] * xs[i])};
-    const auto j = join<LPR, W, true>(own, lds[chunk & 1]);
-    float h = fmaf(j.before.a, state, j.before.b);
-    state = fmaf(j.whole.a, state, j.whole.b);
-    float v[kItems];
+      for (int i = 0; i < kItems<T>; ++i) {
+        xs[i] *= keep[i];
+        own = {own.a * a[i], fmaf(a[i], own.b, xs[i])};
+      }
+      const Joined j = join<LPR, W, true>(own, lds[chunk & 1]);
+      float h = fmaf(j.before.a, state, j.before.b);
+      state = fmaf(j.whole.a, state, j.whole.b);
+      const int s0 = at.start(chunk);
+      float hs[kItems<T>];
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      h = fmaf(a[i], h, keep[i] * xs[i]);
-      const long s = s0 + i;
-      v[i] = (REV ? p.L - 1 - s : s) < len ? h : 0.0f;
-    }
-    if (at.live) store_items<T, REV>(out, s0, p.L, v);
+      for (int i = 0; i < kItems<T>; ++i) {
+        h = fmaf(a[i], h, xs[i]);
+        hs[i] = FULL || at.valid(s0 + i) ? h : 0.0f;
+      }
+      Items<T> v;
+      v.template set<REV>(hs);
+      if (at.live) v.template store<REV>(out, s0, p.L, FULL || at.whole(chunk));
+    });
   }
+  at.blank(out);
   if (at.live && at.lane == 0 && at.seg == p.segments - 1)
     p.last[at.row] = state;
 }
 
-template <typename T, int LPR, int W, bool REV>
-__global__ __launch_bounds__(W > 1 ? W * 64 : 256) void scan_back_kernel(
-    ScanArgs p) {
+SCAN_KERNEL scan_back_kernel(ScanArgs p) {
   __shared__ Map lds[4][W];
-  const Place<LPR, W> at(p);
-  const long n = at.row / p.C, c = at.row % p.C;
-  const int len = valid_length(p, n);
-  const T* x = (const T*)p.x + n * p.xn + c * p.xc;
-  const T* gate = (const T*)p.gate + n * p.gn + c * p.gc;
-  const T* dh = p.dh ? (const T*)p.dh + at.row * p.L : nullptr;
+  const Place<T, LPR, W, REV> at(p);
+  const T *x = at.x(), *gate = at.gate(), *dh = at.dh();
   T* dx = (T*)p.out + at.row * p.L;
   T* dgate = (T*)p.out2 + at.row * p.L;
+  const float* marks = p.marks + at.row * p.chunks;
+  Items<T> xi, gi, di;
+  float mark = 0.0f;
+  auto fetch = [&](int chunk) {
+    const bool whole = at.whole(chunk);
+    gi.template load<REV>(gate, at.start(chunk), p.L, whole);
+    xi.template load<REV>(x, at.start(chunk), p.L, whole);
+    if (dh) di.template load<REV>(dh, at.start(chunk), p.L, whole);
+    mark = marks[chunk];
+  };
+  if (at.begin < at.end) fetch(at.end - 1);
   float u = p.dstate ? p.dstate[at.row] : 0.0f;
   if (p.segments > 1)
     u = through<false>(p.maps + at.row * p.segments * 2, p.segments, at.seg,
                        u);
-  for (int chunk = at.end - 1; chunk >= at.first; --chunk) {
-    const long s0 = ((long)chunk * LPR * W + at.lane) * kItems;
-    const float state = p.marks[at.row * p.chunks + chunk];
-    float xs[kItems], a[kItems], keep[kItems], d[kItems] = {};
-    if (dh) load_items<T, REV>(dh, s0, p.L, d);
-    take<T, REV>(x, gate, s0, p.L, len, xs, a, keep);
-    Map own = {1.0f, 0.0f};
+  for (int chunk = at.end - 1; chunk >= at.begin; --chunk) {
+    for_chunk(at, chunk, [&](auto is_full) {
+      constexpr bool FULL = decltype(is_full)::value;
+      const float state = mark;
+      float xs[kItems<T>], a[kItems<T>], keep[kItems<T>], d[kItems<T>];
+      const Items<T> gn = gi, xn = xi;
 #pragma unroll
-    for (int i = 0; i < kItems; ++i)
-      own = {own.a * a[i], fmaf(a[i], own.b, keep[i] * xs[i])};
-    const auto jf = join<LPR, W, true>(own, lds[chunk & 1]);
-    own = {own.a, 0.0f};
+      for (int i = 0; i < kItems<T>; ++i)
+        d[i] = dh ? di.template at<REV>(i) : 0.0f;
+      if (chunk > at.begin) fetch(chunk - 1);
+      take<REV, FULL>(at, chunk, gn, xn, true, a, keep, xs);
+      const int s0 = at.start(chunk);
+      Map own = {1.0f, 0.0f};
 #pragma unroll
-    for (int i = kItems - 1; i >= 0; --i) {
-      const long s = s0 + i;
-      if ((REV ? p.L - 1 - s : s) >= len) d[i] = 0.0f;
-      own.b = a[i] * (d[i] + own.b);
-    }
-    const auto jb = join<LPR, W, false>(own, lds[2 + (chunk & 1)]);
-    float before[kItems];
-    float h = fmaf(jf.before.a, state, jf.before.b);
+      for (int i = 0; i < kItems<T>; ++i) {
+        if (!FULL && !at.valid(s0 + i)) d[i] = 0.0f;
+        own = {own.a * a[i], fmaf(a[i], own.b, keep[i] * xs[i])};
+      }
+      const Joined jf = join<LPR, W, true>(own, lds[chunk & 1]);
+      own.b = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      before[i] = h;
-      h = fmaf(a[i], h, keep[i] * xs[i]);
-    }
-    float w = fmaf(jb.before.a, u, jb.before.b);
-    u = fmaf(jb.whole.a, u, jb.whole.b);
-    float vx[kItems], vg[kItems];
+      for (int i = kItems<T> - 1; i >= 0; --i) own.b = a[i] * (d[i] + own.b);
+      const Joined jb = join<LPR, W, false>(own, lds[2 + (chunk & 1)]);
+      float before[kItems<T>];
+      float h = fmaf(jf.before.a, state, jf.before.b);
 #pragma unroll
-    for (int i = kItems - 1; i >= 0; --i) {
-      const long s = s0 + i;
-      const bool in = (REV ? p.L - 1 - s : s) < len;
-      const float g = d[i] + w;
-      vx[i] = in ? keep[i] * g : 0.0f;
-      vg[i] = in ? g * (before[i] - xs[i]) * (a[i] * keep[i]) : 0.0f;
-      w = a[i] * g;
-    }
-    if (at.live) {
-      store_items<T, REV>(dx, s0, p.L, vx);
-      store_items<T, REV>(dgate, s0, p.L, vg);
-    }
+      for (int i = 0; i < kItems<T>; ++i) {
+        before[i] = h;
+        h = fmaf(a[i], h, keep[i] * xs[i]);
+      }
+      float w = fmaf(jb.before.a, u, jb.before.b);
+      u = fmaf(jb.whole.a, u, jb.whole.b);
+      Items<T> vx, vg;
+#pragma unroll
+      for (int i = kItems<T> - 1; i >= 0; --i) {
+        const bool in = FULL || at.valid(s0 + i);
+        const float g = d[i] + w;
+        w = a[i] * g;
+        d[i] = in ? keep[i] * g : 0.0f;
+        xs[i] = in ? w * (before[i] - xs[i]) * keep[i] : 0.0f;
+      }
+      vx.template set<REV>(d);
+      vg.template set<REV>(xs);
+      if (at.live) {
+        vx.template store<REV>(dx, s0, p.L, FULL || at.whole(chunk));
+        vg.template store<REV>(dgate, s0, p.L, FULL || at.whole(chunk));
+      }
+    });
   }
-  if (p.last && at.live && at.lane == 0 && at.seg == 0) p.last[at.row] = u;
+  at.blank(dx);
+  at.blank(dgate);
+  if (at.live && at.lane == 0 && at.seg == 0) p.last[at.row] = u;
 }
 
-// How a problem is dealt out. A row gets as many lanes as its length fills;
-// rows longer than a wave's 512 samples get 4 or 16 waves where the rows
-// alone would leave the card short of waves, and segments beyond that.
+#undef SCAN_KERNEL
+
+// How a problem is dealt out. A row gets as many lanes as its length fills.
+// Rows over two waves' samples get 4 waves, which walk the row in longer
+// contiguous pieces (training of (100, 64, 8192) bf16: 71 + 111 us with one
+// wave, 68 + 98 with 4, 66 + 129 with 16, whose waits at the barriers show).
+// Few rows get 16, and are cut into segments until the card has waves enough,
+// two rounds of them (one row set of 24 x 1000003 fp32 in 11, 22 and 43
+// segments: 333, 291 and 300 us).
 struct Deal {
   int lpr, w, chunks, segments, per_segment;
-  Deal(long rows, int L) {
-    lpr = L <= kItems ? 1 : L <= 8 * kItems ? 8 : 64;
+  Deal(long rows, int L, int items) {
+    lpr = L <= items ? 1 : L <= 8 * items ? 8 : 64;
     w = 1;
+    const int wave = 64 * items;
     const long enough = 4096;  // waves
-    if (lpr == 64) {
-      while (w < 16 && rows * w < enough && 64L * kItems * w < L) w *= 4;
-    }
-    chunks = sa::ceil_div(L, lpr * w * kItems);
+    if (L > 2 * wave) w = 4;
+    if (L > 16 * wave && rows * 4 < enough) w = 16;
+    chunks = sa::ceil_div(L, lpr * w * items);
     segments = 1;
     per_segment = chunks;
-    if (lpr == 64 && rows * w < enough / 2 && chunks >= 4) {
-      const long most = std::min<long>(chunks / 2,
-                                       (enough + rows * w - 1) / (rows * w));
+    if (lpr == 64 && rows * w < enough && chunks >= 4) {
+      const long most = std::min<long>(chunks / 2, sa::ceil_div(2 * enough,
+                                                                rows * w));
       per_segment = sa::ceil_div(chunks, most);
       segments = sa::ceil_div(chunks, per_segment);
     }
@@ -505,7 +650,7 @@ std::vector<at::Tensor> forward(const Call& c, bool marked) {
   const long rows = last.numel();
   at::Tensor marks, maps;
   if (rows == 0) return {h, last, marks};
-  const Deal deal(rows, c.x.size(2));
+  const Deal deal(rows, c.x.size(2), 16 / c.x.element_size());
   ScanArgs p = args_of(c, deal);
   if (marked) {
     marks = at::empty({rows, deal.chunks}, f32);
@@ -536,7 +681,7 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& marks,
   auto first = at::empty({c.x.size(0), c.x.size(1)}, f32);
   const long rows = first.numel();
   if (rows == 0) return {dx, dgate, first};
-  const Deal deal(rows, c.x.size(2));
+  const Deal deal(rows, c.x.size(2), 16 / c.x.element_size());
   ScanArgs p = args_of(c, deal);
   if (dh.defined()) p.dh = dh.data_ptr();
   if (dstate.defined()) p.dstate = dstate.data_ptr<float>();
