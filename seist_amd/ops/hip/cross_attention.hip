@@ -81,7 +81,9 @@ __device__ __forceinline__ void weigh(float (&s)[SUBS][16], float scale,
 // half of the matrix rate.
 template <typename T, int ED, int QB, int POS, bool BIASED>
 __global__ __launch_bounds__(
-    256, ED * QB * (BIASED ? 2 : 1) * sizeof(T) <= 256 ? 2 : 1) void
+    256, ED * QB * sizeof(T) <= 64                     ? 4
+         : ED * QB * (BIASED ? 2 : 1) * sizeof(T) <= 256 ? 2
+                                                         : 1) void
 attend_kernel(Args p) {
   using M = Mma<T>;
   using Staged = Tile<T, ED, POS, 256>;
@@ -106,6 +108,17 @@ attend_kernel(Args p) {
   const int begin = split * p.per_split;
   const int end = min(total, begin + p.per_split);
 
+  const float scale = p.scale * kLog2e;
+  const T* kb = (const T*)p.k + n * p.kn + hk * p.kh;
+  const T* vb = (const T*)p.v + n * p.vn + hk * p.vh;
+  Staged ks, vs;
+  ks.place(p.ke, p.E, tid);
+  vs.place(p.ve, p.E, tid);
+  if (begin < end) {
+    ks.load(kb, begin, end, tid);
+    vs.load(vb, begin, end, tid);
+  }
+
   float* line = (float*)(shared + 4 * Staged::kBytes) +
                 line_middle(p.bias.max_distance, false);
   float before = 0.0f, behind = 0.0f;
@@ -123,25 +136,14 @@ attend_kernel(Args p) {
                        (const T*)p.q + n * p.qn + head * p.qh, p.qe, p.E,
                        first - g * p.pad + 32 * c, p.Lq);
   __syncthreads();
+  if (p.E < ED)
+    for (int b = 0; b < 4; ++b)
+      Staged::blank((T*)(shared + b * Staged::kBytes), p.E, tid);
 
   f32x16 acc[QB][DB] = {};
   float most[QB], sum[QB];
 #pragma unroll
   for (int c = 0; c < QB; ++c) most[c] = -INFINITY, sum[c] = 0.0f;
-  const float scale = p.scale * kLog2e;
-  const T* kb = (const T*)p.k + n * p.kn + hk * p.kh;
-  const T* vb = (const T*)p.v + n * p.vn + hk * p.vh;
-
-  Staged ks, vs;
-  ks.place(p.ke, p.E, tid);
-  vs.place(p.ve, p.E, tid);
-  if (begin < end) {
-    ks.load(kb, begin, end, tid);
-    vs.load(vb, begin, end, tid);
-    if (p.E < ED)
-      for (int b = 0; b < 4; ++b)
-        Staged::blank((T*)(shared + b * Staged::kBytes), p.E, tid);
-  }
   int buf = 0;
   for (int at = begin; at < end; at += POS, buf ^= 1) {
     T* kt = (T*)(shared + 2 * buf * Staged::kBytes);
@@ -297,6 +299,18 @@ attend_few_kernel(Args p) {
 
   T* kt = (T*)(shared + wave * BYTES);
   T* vt = (T*)(shared + wave * BYTES + Staged::kBytes);
+  const float scale = p.scale * kLog2e;
+  const T* kb = (const T*)p.k + n * p.kn + hk * p.kh;
+  const T* vb = (const T*)p.v + n * p.vn + hk * p.vh;
+
+  Staged ks, vs;
+  int at = begin + 32 * wave;
+  ks.place(p.ke, p.E, lane);
+  vs.place(p.ve, p.E, lane);
+  if (at < end) {
+    ks.load(kb, at, end, lane);
+    vs.load(vb, at, end, lane);
+  }
   float* stats = (float*)(shared + 4 * BYTES);  // (4, 2, 32)
   float* table = stats + 256;                   // (G, buckets), log2
   unsigned char* ids =                          // buckets by distance
@@ -319,13 +333,14 @@ attend_few_kernel(Args p) {
   typename M::Op q[ED / M::kDepth];
   {
     T* qt = (T*)shared;  // (ED, 32), the rows as columns
-    for (int c = threadIdx.x; c < ED * 32; c += 256) {
-      const int e = c / 32, r = c % 32;
-      T v = (T)0.0f;
-      if (e < p.E && r < rows)
-        v = ((const T*)p.q)[n * p.qn + (hk * p.G + r / p.Lq) * p.qh +
-                            e * p.qe + r % p.Lq];
-      qt[e * Staged::kStride + r] = v;
+    const int r = threadIdx.x & 31, from = min(r, rows - 1);
+    const T* p0 = (const T*)p.q + n * p.qn +
+                  (hk * p.G + from / p.Lq) * p.qh + from % p.Lq;
+#pragma unroll
+    for (int o = 0; o < ED / 8; ++o) {
+      const int e = o * 8 + (threadIdx.x >> 5);
+      const T v = p0[min(e, p.E - 1) * p.qe];
+      qt[e * Staged::kStride + r] = e < p.E && r < rows ? v : (T)0.0f;
     }
     __syncthreads();
 #pragma unroll
@@ -335,21 +350,9 @@ attend_few_kernel(Args p) {
   }
   f32x16 acc[DB] = {};
   float most = -INFINITY, sum = 0.0f;
-  const float scale = p.scale * kLog2e;
-  const T* kb = (const T*)p.k + n * p.kn + hk * p.kh;
-  const T* vb = (const T*)p.v + n * p.vn + hk * p.vh;
-
-  Staged ks, vs;
-  int at = begin + 32 * wave;
-  ks.place(p.ke, p.E, lane);
-  vs.place(p.ve, p.E, lane);
-  if (at < end) {
-    ks.load(kb, at, end, lane);
-    vs.load(vb, at, end, lane);
-    if (p.E < ED) {
-      Staged::blank(kt, p.E, lane);
-      Staged::blank(vt, p.E, lane);
-    }
+  if (p.E < ED && at < end) {
+    Staged::blank(kt, p.E, lane);
+    Staged::blank(vt, p.E, lane);
   }
   for (; at < end; at += 128) {
     wave_fence();

@@ -23,8 +23,8 @@ size_t deep_lds(size_t lines) {
   return std::max<size_t>(staged, 8 * Columns<T, ED>::kBytes);
 }
 
-// A workgroup's sums of ds by distance (a line for each of its 8 half waves)
-// and beyond the last one (a wave's in each lane), added up by bucket, each
+// A workgroup's sums of ds by distance (a line for each of its 4 waves) and
+// beyond the last one (a wave's in each lane), added up by bucket, each
 // in the same order every time. `ends`: 8 floats of LDS.
 __device__ __forceinline__ void fold_table(const Bias& b, const float* lines,
                                            float before, float behind,
@@ -55,11 +55,53 @@ __device__ __forceinline__ void fold_table(const Bias& b, const float* lines,
     for (int n = lo + lane; n < hi; n += 64) {
       const int d = b.max_distance + (after ? n : -n);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v += lines[k * wide + d];
+      for (int k = 0; k < 4; ++k) v += lines[k * wide + d];
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
     if (lane == 0) out[at] = v;
+  }
+}
+
+// Adds a wave's ds, 32 keys by 32 queries, to its sums by distance. Adding
+// them where they are, an atomic an element, took 224 cycles for 64 lanes; so
+// they go through LDS, and a lane sums a whole diagonal of equal distances:
+// each distance is then added to once, in the same order every time.
+template <typename T>
+__device__ __forceinline__ void add_diagonals(const Bias& b,
+                                              const float (&ds)[16],
+                                              float* tile, float* sums,
+                                              int d0, float& before,
+                                              float& behind) {
+  using M = Mma<T>;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const int step = b.key_step, far = b.max_distance;
+  auto add = [&](int d, float v) {
+    before += d <= -far ? v : 0.0f;
+    behind += d >= far ? v : 0.0f;
+    if (d > -far && d < far) sums[d] += v;
+  };
+  if (step >= 32) {  // no two of the tile's distances are equal
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      add(d0 + M::seq(j, h) * step - (lane & 31), ds[j]);
+    return;
+  }
+  constexpr int STRIDE = 33;  // a diagonal's reads then fall on other banks
+  wave_fence();
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    tile[M::seq(j, h) * STRIDE + (lane & 31)] = ds[j];
+  wave_fence();
+  const float inv = 1.0f / step;
+  // r = key * step - query, both within the tile
+  for (int r = lane - 31; r <= 31 * step; r += 64) {
+    // whole quotients: half a unit is more than what the products are off
+    const int from = r > 0 ? (int)((r + step - 0.5f) * inv) : 0;
+    const int to = min(31, (int)((r + 31.5f) * inv));
+    float v = 0.0f;
+    for (int k = from; k <= to; ++k) v += tile[k * STRIDE + k * step - r];
+    add(d0 + r, v);
   }
 }
 
@@ -123,19 +165,19 @@ void attend_dq_kernel(Args p) {
 
   float* line = (float*)(shared + 4 * Staged::kBytes) +
                 line_middle(far, false);
-  // the wave's ds by distance, a line for each of its halves
-  float* lines = line + far + 1 + wave * 2 * (2 * far + 1);
+  float* lines = line + far + 1;  // the waves' ds by distance
+  float* ends = lines + 4 * (2 * far + 1);
+  float* diagonals = ends + 8 + wave * 32 * 33;
   float before = 0.0f, behind = 0.0f;      // bias past the last bucket
   float ds_before = 0.0f, ds_behind = 0.0f;
   if (LINED) {  // the workgroup's rows are one head's
     spread_bias<T, false>(p.bias, head, line, tid, 256);
     before = bias_of<T>(p.bias, head, -far);
     behind = bias_of<T>(p.bias, head, far);
-    if (TABLE) {
-      for (int d = lane; d < 2 * (2 * far + 1); d += 64) lines[d] = 0.0f;
-    }
+    if (TABLE)
+      for (int d = tid; d < 4 * (2 * far + 1); d += 256) lines[d] = 0.0f;
   }
-  float* sums = lines + h * (2 * far + 1) + far;
+  float* sums = lines + wave * (2 * far + 1) + far;
 
   f32x16 acc[DB] = {};
   const float scale = p.scale * kLog2e;
@@ -213,18 +255,9 @@ void attend_dq_kernel(Args p) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) ds[j] *= dp[j] - delta;
         if (TABLE && side == 0) {
-          // the lanes of a half have different distances, and a wave's
-          // additions reach LDS in order: the sums come out the same each
-          // time
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int d = d0 + M::seq(j, 0) * p.bias.key_step;
-            ds_before += d <= -far ? ds[j] : 0.0f;
-            ds_behind += d >= far ? ds[j] : 0.0f;
-            if (d > -far && d < far)
-              __hip_atomic_fetch_add(sums + d, ds[j], __ATOMIC_RELAXED,
-                                     __HIP_MEMORY_SCOPE_WORKGROUP);
-          }
+          add_diagonals<T>(p.bias, ds, diagonals, sums,
+                           key0 * p.bias.key_step - from, ds_before,
+                           ds_behind);
         } else if (TABLE) {
           float all = 0.0f;
 #pragma unroll
@@ -245,8 +278,7 @@ void attend_dq_kernel(Args p) {
   }
   const int rows = p.G * p.pad;
   if (TABLE)  // a workgroup's rows are one head's, and there are some
-    fold_table(p.bias, line + far + 1, ds_before, ds_behind,
-               line + far + 1 + 8 * (2 * far + 1),
+    fold_table(p.bias, lines, ds_before, ds_behind, ends,
                p.dbias + (((long)(n * p.splits + split) * p.H + head) *
                               (p.pad / 128) + i0 / 128) * p.bias.buckets);
   if (first >= rows || !live) return;
@@ -617,18 +649,18 @@ __global__ __launch_bounds__(256) void sum_table_kernel(const float* in,
                                                         int buckets) {
   __shared__ float sums[4][kMaxBuckets];
   const int b = threadIdx.x & 63, lane = threadIdx.x >> 6;
-  const long rows = (long)N * tiles;
-  const long each = (rows + gridDim.y - 1) / gridDim.y;
-  const long begin = blockIdx.y * each, end = min(rows, begin + each);
+  const int rows = N * tiles;
+  const int each = (rows + gridDim.y - 1) / gridDim.y;
+  const int begin = blockIdx.y * each, end = min(rows, begin + each);
   float v = 0.0f;
   // 8 rows at a time, so that their loads are on the way together
-  for (long r0 = begin + lane; r0 < end && b < buckets; r0 += 32) {
+  for (int r0 = begin + lane; r0 < end && b < buckets; r0 += 32) {
     float w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const long r = min(r0 + 4 * i, end - 1);
-      w[i] = in[((r / tiles * H + blockIdx.x) * tiles + r % tiles) * buckets +
-                b];
+      const int r = min(r0 + 4 * i, end - 1), n = r / tiles;
+      w[i] = in[(((long)n * H + blockIdx.x) * tiles + r - n * tiles) *
+                    buckets + b];
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) v += r0 + 4 * i < end ? w[i] : 0.0f;
@@ -694,7 +726,7 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
       const long blocks = pairs * p.splits * p.tiles;
       if (table)
         launch(attend_dq_kernel<T, ED, POS, true, true>, blocks, 256,
-               backward_lds<T, ED>(9 * line + 32), p, stream);
+               backward_lds<T, ED>(5 * line + 32 + 4 * 32 * 33 * 4), p, stream);
       else if (p.bias.table)
         launch(attend_dq_kernel<T, ED, POS, true, false>, blocks, 256,
                backward_lds<T, ED>(line), p, stream);

@@ -550,7 +550,7 @@ SCAN_KERNEL scan_back_kernel(ScanArgs p) {
 struct Deal {
   int lpr, w, chunks, segments, per_segment;
   Deal(long rows, int L, int items) {
-    lpr = L <= items ? 1 : L <= 8 * items ? 8 : 64;
+    lpr = L <= items ? 1 : L <= 16 * items ? 16 : 64;
     w = 1;
     const int wave = 64 * items;
     const long enough = 4096;  // waves
@@ -599,7 +599,7 @@ template <typename T, bool REV>
 void launch_rev(Which which, const ScanArgs& p, const Deal& deal,
                 hipStream_t stream) {
   if (deal.lpr == 1) launch_one<T, 1, 1, REV>(which, p, deal, stream);
-  else if (deal.lpr == 8) launch_one<T, 8, 1, REV>(which, p, deal, stream);
+  else if (deal.lpr == 16) launch_one<T, 16, 1, REV>(which, p, deal, stream);
   else if (deal.w == 1) launch_one<T, 64, 1, REV>(which, p, deal, stream);
   else if (deal.w == 4) launch_one<T, 64, 4, REV>(which, p, deal, stream);
   else launch_one<T, 64, 16, REV>(which, p, deal, stream);
