@@ -7,6 +7,8 @@
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 
+#include <climits>
+
 #include "sa_common.h"
 
 namespace attend {
@@ -26,8 +28,8 @@ constexpr float kOut = -1e30f;
 
 struct Bias {
   const void* table;  // (H, buckets), null without
-  int buckets, exact, steps, max_distance, key_step, query_start;
-  int threshold[kMaxThresholds];
+  int buckets, exact, max_distance, key_step, query_start;
+  int threshold[kMaxThresholds];  // those there are not: INT_MAX
 };
 
 struct Args {
@@ -43,6 +45,7 @@ struct Args {
   int N, H, Hkv, G, E, Lq, Lk;
   int pad;         // rows a head takes: Lq, or Lq rounded up to whole tiles
   int tiles;       // row (or key) tiles of a workgroup's size
+  int runs;        // row tiles that a workgroup takes one after another
   int splits, per_split;
   float scale;     // times log2(e) in the scores, plain in the gradients
   Bias bias;
@@ -293,7 +296,8 @@ __device__ __forceinline__ int bucket_of(const Bias& b, int d) {
   int at = n;
   if (n >= b.exact) {
     at = b.exact;
-    for (int m = 0; m < b.steps; ++m) at += n >= b.threshold[m];
+#pragma unroll
+    for (int m = 0; m < kMaxThresholds; ++m) at += n >= b.threshold[m];
   }
   return d > 0 ? at + b.buckets / 2 : at;
 }
@@ -438,11 +442,12 @@ inline Args args_of(const Call& c) {
     b.table = c.table.data_ptr();
     b.buckets = c.table.size(1);
     b.exact = b.buckets / 4;
-    b.steps = c.thresholds.size();
     b.max_distance = c.max_distance;
     b.key_step = c.key_step;
     b.query_start = c.query_start;
-    for (int m = 0; m < b.steps; ++m) b.threshold[m] = c.thresholds[m];
+    for (int m = 0; m < kMaxThresholds; ++m)
+      b.threshold[m] = m < (int)c.thresholds.size() ? c.thresholds[m]
+                                                    : INT_MAX;
   }
   return p;
 }

@@ -6,6 +6,8 @@ Produces seist_amd/_C.*.so next to the package so the GPU-box snapshot
 carries it (no JIT cache dependence).
 """
 
+import glob
+import hashlib
 import os
 
 from setuptools import setup
@@ -17,6 +19,13 @@ from setuptools import Extension  # noqa: E402
 from torch.utils.cpp_extension import BuildExtension, CUDAExtension  # noqa: E402
 
 HIP_DIR = os.path.join("seist_amd", "ops", "hip")
+
+# Every kernel source is compiled with this, so that all of them are compiled
+# again when a header they share changes: the object rules name no headers,
+# and objects that disagree on a struct's layout fault the GPU.
+HEADERS = hashlib.md5(b"".join(
+    open(h, "rb").read() for h in sorted(glob.glob(os.path.join(HIP_DIR, "*.h")))
+    if not h.endswith("_hip.h"))).hexdigest()
 
 # K20: plain-C++ data-pipeline workers (no HIP/torch dependency — runs in
 # DataLoader worker processes)
@@ -56,7 +65,7 @@ ext = CUDAExtension(
         "cxx": ["-O3", "-std=c++17"],
         # packed fp32 instructions stay off: plain float code only
         "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
-                 "-Xclang", "-packed-fp32-ops"],
+                 "-Xclang", "-packed-fp32-ops", f"-DSA_HEADERS={HEADERS}"],
     },
 )
 

@@ -59,6 +59,8 @@ def _check_attention(q, k, v, do, table, lens=None, **more):
     (1, 1, 1, 33, 1, 2500),     # a long split of the keys
     (1, 1, 1, 17, 2500, 3),     # few keys: a long split of the queries
     (3, 33, 1, 8, 1, 40),       # 33 heads share a key head
+    (8, 16, 16, 8, 1050, 100),  # few keys, rows enough for several a workgroup
+    (8, 32, 16, 24, 600, 128),  # the same, across heads that share keys
 ])
 def test_attention(dtype, n, h, hkv, e, lq, lk):
     _check_attention(*_attention_inputs(n, h, hkv, e, lq, lk, 0, dtype))
@@ -74,6 +76,7 @@ def test_attention(dtype, n, h, hkv, e, lq, lk):
     (1, 1, 1, 128, 70, 200, 4, dict(max_distance=2, query_start=-50)),
     (1, 2, 1, 80, 65, 150, 6, dict(max_distance=1000, key_step=3)),
     (2, 2, 2, 16, 300, 500, 32, dict(max_distance=9, scale=0.3)),
+    (8, 32, 16, 8, 600, 100, 8, dict(max_distance=100, key_step=6)),
 ])
 def test_attention_with_bias(dtype, n, h, hkv, e, lq, lk, buckets, more):
     _check_attention(*_attention_inputs(n, h, hkv, e, lq, lk, buckets, dtype),
