@@ -45,7 +45,6 @@ struct Args {
   int N, H, Hkv, G, E, Lq, Lk;
   int pad;         // rows a head takes: Lq, or Lq rounded up to whole tiles
   int tiles;       // row (or key) tiles of a workgroup's size
-  int runs;        // row tiles that a workgroup takes one after another
   int splits, per_split;
   float scale;     // times log2(e) in the scores, plain in the gradients
   Bias bias;
@@ -323,6 +322,29 @@ __host__ __device__ inline int line_floats(int max_distance, bool padded) {
 __host__ __device__ inline int line_middle(int max_distance, bool padded) {
   return max_distance + (padded ? max_distance / 16 + 1 : 0);
 }
+
+// A line in LDS by the address that an entry has: 4 times the distance from
+// distance 0's, held to the line's ends, so that a score's bias costs an
+// addition, a comparison of three and the load. Distances stay under 2^28.
+struct Line {
+  int zero, low, high;
+  __device__ __forceinline__ Line(const float* middle, int most) {
+    zero = (int)(size_t)(const __attribute__((address_space(3))) float*)
+        middle;
+    low = zero - 4 * most;
+    high = zero + 4 * most;
+  }
+  __device__ __forceinline__ int at(int distance) const {
+    return zero + 4 * distance;
+  }
+  __device__ __forceinline__ float get(int at) const {
+    int held;
+    asm("v_med3_i32 %0, %1, %2, %3"
+        : "=v"(held)
+        : "v"(at), "v"(low), "v"(high));
+    return *(const __attribute__((address_space(3))) float*)(size_t)held;
+  }
+};
 
 // 32 columns of queries (or keys) against `span` positions of the other
 // sequence: whether every distance is past the last bucket's start. `least`

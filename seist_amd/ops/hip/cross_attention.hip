@@ -79,7 +79,7 @@ __device__ __forceinline__ void weigh(float (&s)[SUBS][16], float scale,
 // 4 x QB x 32 rows. Two blocks of 32 columns for a wave (QB = 2) read a
 // tile's operands from LDS once for both; LDS reads bound one block at about
 // half of the matrix rate.
-template <typename T, int ED, int QB, int POS, bool BIASED, bool RUNS>
+template <typename T, int ED, int QB, int POS, bool BIASED>
 __global__ __launch_bounds__(
     256, ED * QB * (BIASED ? 2 : 1) * sizeof(T) <= 256 ? 2 : 1) void
 attend_kernel(Args p) {
@@ -114,174 +114,149 @@ attend_kernel(Args p) {
 
   float* line = (float*)(shared + 4 * Staged::kBytes) +
                 line_middle(p.bias.max_distance, false);
-  // where the columns pass through: the staged tiles' place, or behind
-  // everything else where those are to stay
-  T* pass = (T*)shared + wave * (Columns<T, ED>::kBytes / sizeof(T));
-  if (RUNS)
-    pass += (4 * Staged::kBytes +
-             (BIASED ? line_floats(p.bias.max_distance, false) / 4 * 16 + 16
-                     : 0)) /
-            sizeof(T);
-  int lined = -1;
+  const int first = (tile * 4 + wave) * 32 * QB;  // this wave's first row
+  const int g = min(first / p.pad, p.G - 1);
+  const int head = hk * p.G + g;
+  const int i0 = first - g * p.pad + (lane & 31);
   float before = 0.0f, behind = 0.0f;
-  const int runs = RUNS ? p.runs : 1;
+  if (BIASED) {  // the workgroup's rows are one head's
+    spread_bias<T, false>(p.bias, head, line, tid, 256);
+    before = bias_of<T>(p.bias, head, -p.bias.max_distance);
+    behind = bias_of<T>(p.bias, head, p.bias.max_distance);
+  }
+  typename M::Op q[QB][ED / M::kDepth];
+#pragma unroll
+  for (int c = 0; c < QB; ++c)
+    own_columns<T, ED>(q[c], (T*)shared + wave * (Columns<T, ED>::kBytes / sizeof(T)),
+                       (const T*)p.q + n * p.qn + head * p.qh, p.qe, p.E,
+                       first - g * p.pad + 32 * c, p.Lq);
+  __syncthreads();
+  if (p.E < ED)
+    for (int b = 0; b < 4; ++b)
+      Staged::blank((T*)(shared + b * Staged::kBytes), p.E, tid);
 
-  // Where one staged tile holds all keys, a workgroup takes several row tiles
-  // to it one after another (p.runs).
+  const Line bias_line(line, p.bias.max_distance);
+  f32x16 acc[QB][DB] = {};
+  float most[QB], sum[QB];
+#pragma unroll
+  for (int c = 0; c < QB; ++c) most[c] = -INFINITY, sum[c] = 0.0f;
+  int buf = 0;
+  for (int at = begin; at < end; at += POS, buf ^= 1) {
+    T* kt = (T*)(shared + 2 * buf * Staged::kBytes);
+    T* vt = (T*)(shared + (2 * buf + 1) * Staged::kBytes);
+    ks.store(kt, p.E, tid);
+    vs.store(vt, p.E, tid);
+    __syncthreads();
+    if (at + POS < end) {
+      ks.load(kb, at + POS, end, tid);
+      vs.load(vb, at + POS, end, tid);
+    }
+    if (first - g * p.pad >= p.Lq) continue;  // no query of this wave's
 #pragma unroll 1
-  for (int run = 0; run < runs; ++run) {
-    int length = p.Lq;  // the results' places are made anew for each run,
-    if (RUNS) asm volatile("" : "+s"(length));  // not kept in registers
-    const int first = ((tile * runs + run) * 4 + wave) * 32 * QB;
-    const int g = min(first / p.pad, p.G - 1);
-    const int head = hk * p.G + g;
-    const int i0 = first - g * p.pad + (lane & 31);
-    if (BIASED && g != lined) {  // the workgroup's rows are one head's
-      if (run > 0) __syncthreads();
-      spread_bias<T, false>(p.bias, head, line, tid, 256);
-      before = bias_of<T>(p.bias, head, -p.bias.max_distance);
-      behind = bias_of<T>(p.bias, head, p.bias.max_distance);
-      if (run > 0) __syncthreads();
-      lined = g;
-    }
-    typename M::Op q[QB][ED / M::kDepth];
+    for (int col = 0; col < POS && at + col < end; col += STEP) {
+      const int key0 = at + col;
+      float s[QB][SUBS][16];
 #pragma unroll
-    for (int c = 0; c < QB; ++c)
-      own_columns<T, ED>(q[c], pass,
-                         (const T*)p.q + n * p.qn + head * p.qh, p.qe, p.E,
-                         first - g * p.pad + 32 * c, p.Lq);
-    if (run == 0) {
-      __syncthreads();
-      if (p.E < ED)
-        for (int b = 0; b < 4; ++b)
-          Staged::blank((T*)(shared + b * Staged::kBytes), p.E, tid);
-    }
-
-    f32x16 acc[QB][DB] = {};
-    float most[QB], sum[QB];
+      for (int b = 0; b < SUBS; ++b) {
+        f32x16 c[QB] = {};
 #pragma unroll
-    for (int c = 0; c < QB; ++c) most[c] = -INFINITY, sum[c] = 0.0f;
-    int buf = 0;
-    for (int at = begin; at < end; at += POS, buf ^= 1) {
-      T* kt = (T*)(shared + 2 * buf * Staged::kBytes);
-      T* vt = (T*)(shared + (2 * buf + 1) * Staged::kBytes);
-      if (run == 0) {
-        ks.store(kt, p.E, tid);
-        vs.store(vt, p.E, tid);
-        __syncthreads();
+        for (int kk = 0; kk < ED / M::kDepth; ++kk) {
+          const auto a = M::template first<Staged::kStride>(kt, kk, col + 32 * b);
+#pragma unroll
+          for (int o = 0; o < QB; ++o) c[o] = M::mul(a, q[o][kk], c[o]);
+        }
+#pragma unroll
+        for (int o = 0; o < QB; ++o)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[o][b][j] = c[o][j];
       }
-      if (at + POS < end) {
-        ks.load(kb, at + POS, end, tid);
-        vs.load(vb, at + POS, end, tid);
+      if (key0 + STEP > end) {
+#pragma unroll
+        for (int b = 0; b < SUBS; ++b)
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (key0 + 32 * b + M::seq(j, h) >= end)
+#pragma unroll
+              for (int o = 0; o < QB; ++o) s[o][b][j] = -INFINITY;
       }
-      if (first - g * p.pad >= p.Lq) continue;  // no query of this wave's
-#pragma unroll 1
-      for (int col = 0; col < POS && at + col < end; col += STEP) {
-        const int key0 = at + col;
-        float s[QB][SUBS][16];
+      int side = 2;
+      if (BIASED) {
+        const int from = first - g * p.pad + p.bias.query_start;
+        side = beyond(p.bias, key0 * p.bias.key_step - (from + 32 * QB - 1),
+                      (key0 + STEP - 1) * p.bias.key_step - from);
+      }
+      if (BIASED && side == 0) {
 #pragma unroll
-        for (int b = 0; b < SUBS; ++b) {
-          f32x16 c[QB] = {};
+        for (int o = 0; o < QB; ++o) {
+          // the lane's own part of a distance; the rest is the wave's
+        const int a0 = bias_line.at((key0 + M::seq(0, h)) * p.bias.key_step -
+                                    (i0 + 32 * o + p.bias.query_start));
 #pragma unroll
-          for (int kk = 0; kk < ED / M::kDepth; ++kk) {
-            const auto a = M::template first<Staged::kStride>(kt, kk, col + 32 * b);
+        for (int b = 0; b < SUBS; ++b)
 #pragma unroll
-            for (int o = 0; o < QB; ++o) c[o] = M::mul(a, q[o][kk], c[o]);
-          }
-#pragma unroll
-          for (int o = 0; o < QB; ++o)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) s[o][b][j] = c[o][j];
+          for (int j = 0; j < 16; ++j)
+            s[o][b][j] = fmaf(
+                s[o][b][j], scale,
+                bias_line.get(a0 + 4 * (32 * b + M::seq(j, 0)) *
+                                       p.bias.key_step));
+        weigh<SUBS, DB, true>(s[o], 1.0f, 0.0f, most[o], sum[o], acc[o]);
         }
-        if (key0 + STEP > end) {
+      } else {
+        const float add = !BIASED ? 0.0f : side > 0 ? behind : before;
 #pragma unroll
-          for (int b = 0; b < SUBS; ++b)
+        for (int o = 0; o < QB; ++o)
+          weigh<SUBS, DB, false>(s[o], scale, add, most[o], sum[o], acc[o]);
+      }
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (key0 + 32 * b + M::seq(j, h) >= end)
+      for (int b = 0; b < SUBS; ++b) {
+        typename M::Right pr[QB];
 #pragma unroll
-                for (int o = 0; o < QB; ++o) s[o][b][j] = -INFINITY;
-        }
-        int side = 2;
-        if (BIASED) {
-          const int from = first - g * p.pad + p.bias.query_start;
-          side = beyond(p.bias, key0 * p.bias.key_step - (from + 32 * QB - 1),
-                        (key0 + STEP - 1) * p.bias.key_step - from);
-        }
-        if (BIASED && side == 0) {
+        for (int o = 0; o < QB; ++o) M::right(pr[o], s[o][b]);
 #pragma unroll
-          for (int o = 0; o < QB; ++o) {
-            // the lane's own part of a distance; the rest is the wave's
-            const int d0 = (key0 + M::seq(0, h)) * p.bias.key_step -
-                           (i0 + 32 * o + p.bias.query_start);
+        for (int d = 0; d < DB; ++d) {
+          const auto a =
+              M::template second<Staged::kStride, ED>(vt, 32 * d, col + 32 * b);
 #pragma unroll
-            for (int b = 0; b < SUBS; ++b)
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const int d = d0 + (32 * b + M::seq(j, 0)) * p.bias.key_step;
-                s[o][b][j] = fmaf(
-                    s[o][b][j], scale,
-                    line[max(-p.bias.max_distance, min(d, p.bias.max_distance))]);
-              }
-            weigh<SUBS, DB, true>(s[o], 1.0f, 0.0f, most[o], sum[o], acc[o]);
-          }
-        } else {
-          const float add = !BIASED ? 0.0f : side > 0 ? behind : before;
-#pragma unroll
-          for (int o = 0; o < QB; ++o)
-            weigh<SUBS, DB, false>(s[o], scale, add, most[o], sum[o], acc[o]);
-        }
-#pragma unroll
-        for (int b = 0; b < SUBS; ++b) {
-          typename M::Right pr[QB];
-#pragma unroll
-          for (int o = 0; o < QB; ++o) M::right(pr[o], s[o][b]);
-#pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            const auto a =
-                M::template second<Staged::kStride, ED>(vt, 32 * d, col + 32 * b);
-#pragma unroll
-            for (int o = 0; o < QB; ++o) acc[o][d] = M::mul(a, pr[o], acc[o][d]);
-          }
+          for (int o = 0; o < QB; ++o) acc[o][d] = M::mul(a, pr[o], acc[o][d]);
         }
       }
     }
+  }
 
 #pragma unroll
-    for (int o = 0; o < QB; ++o) {
-      const float all = both_sum(sum[o]);
-      const int i = i0 + 32 * o;
-      if (i >= p.Lq || first >= p.G * p.pad) continue;
-      if (p.splits > 1) {
-        const int rows = p.G * p.pad, row = first + 32 * o + (lane & 31);
-        const long at = (long)split * p.N * p.Hkv + nh;
-        float* out = p.part + at * p.E * rows + row;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int e = 32 * d + 8 * (j / 4) + 4 * h + j % 4;
-            if (e < p.E) out[(long)e * rows] = acc[o][d][j];
-          }
-        if (h == 0) {
-          p.stat[(at * 2 + 0) * rows + row] = most[o];
-          p.stat[(at * 2 + 1) * rows + row] = all;
-        }
-        continue;
-      }
-      const float inv = all > 0.0f ? 1.0f / all : all;  // 0 stays, NaN stays
-      T* out = (T*)p.out + ((long)n * p.H + head) * p.E * length + i;
+  for (int o = 0; o < QB; ++o) {
+    const float all = both_sum(sum[o]);
+    const int i = i0 + 32 * o;
+    if (i >= p.Lq || first >= p.G * p.pad) continue;
+    if (p.splits > 1) {
+      const int rows = p.G * p.pad, row = first + 32 * o + (lane & 31);
+      const long at = (long)split * p.N * p.Hkv + nh;
+      float* out = p.part + at * p.E * rows + row;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int e = 32 * d + 8 * (j / 4) + 4 * h + j % 4;
-          if (e < p.E) out[(long)e * length] = (T)(acc[o][d][j] * inv);
+          if (e < p.E) out[(long)e * rows] = acc[o][d][j];
         }
-      if (p.lse && h == 0)
-        p.lse[((long)n * p.H + head) * p.Lq + i] =
-            all == 0.0f ? INFINITY : most[o] + log2f(all);
+      if (h == 0) {
+        p.stat[(at * 2 + 0) * rows + row] = most[o];
+        p.stat[(at * 2 + 1) * rows + row] = all;
+      }
+      continue;
     }
+    const float inv = all > 0.0f ? 1.0f / all : all;  // 0 stays, NaN stays
+    T* out = (T*)p.out + ((long)n * p.H + head) * p.E * p.Lq + i;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int e = 32 * d + 8 * (j / 4) + 4 * h + j % 4;
+        if (e < p.E) out[(long)e * p.Lq] = (T)(acc[o][d][j] * inv);
+      }
+    if (p.lse && h == 0)
+      p.lse[((long)n * p.H + head) * p.Lq + i] =
+          all == 0.0f ? INFINITY : most[o] + log2f(all);
   }
 }
 
@@ -517,38 +492,17 @@ __global__ __launch_bounds__(64) void attend_join_kernel(Args p) {
         sum == 0.0f ? INFINITY : most + log2f(sum);
 }
 
-template <typename T, int ED, int QB, bool RUNS>
-void launch_attend(const Args& p, hipStream_t stream) {
+template <typename T, int ED, int QB>
+void launch_attend(const Args& p, long blocks, hipStream_t stream) {
   constexpr int POS = tile_positions<T, ED>();
-  const long blocks = (long)p.N * p.Hkv * p.splits * p.tiles;
-  const size_t lds = 4 * Tile<T, ED, POS, 256>::kBytes +
-                     (RUNS ? 4 * Columns<T, ED>::kBytes : 0);
+  const size_t lds = 4 * Tile<T, ED, POS, 256>::kBytes;
   if constexpr (QB == 1) {
     if (p.bias.table)
-      return launch(attend_kernel<T, ED, 1, POS, true, RUNS>, blocks, 256,
-                    lds + line_floats(p.bias.max_distance, false) / 4 * 16 +
-                        16,
-                    p, stream);
+      return launch(attend_kernel<T, ED, 1, POS, true>, blocks, 256,
+                    lds + 4 * line_floats(p.bias.max_distance, false), p,
+                    stream);
   }
-  launch(attend_kernel<T, ED, QB, POS, false, RUNS>, blocks, 256, lds, p,
-         stream);
-}
-
-template <typename T, int ED, int QB>
-void launch_attend(Args p, hipStream_t stream) {
-  if constexpr (ED * sizeof(T) <= 64) {
-    // two workgroups to a compute unit: the staging, and the bias by
-    // distance, are then made once for all rows that a workgroup has
-    // (queries of 64 x 3 heads of 8, 2048 each, to 128 keys with a bias:
-    // 39 us with a workgroup for each 128 of them)
-    const long all = (long)p.N * p.Hkv * p.tiles;
-    if (p.Lk <= tile_positions<T, ED>() && p.splits == 1 && all >= 2 * 512) {
-      p.runs = std::min<long>(p.tiles, all / 512);
-      p.tiles = sa::ceil_div(p.tiles, p.runs);
-      return launch_attend<T, ED, QB, true>(p, stream);
-    }
-  }
-  launch_attend<T, ED, QB, false>(p, stream);
+  launch(attend_kernel<T, ED, QB, POS, false>, blocks, 256, lds, p, stream);
 }
 
 std::vector<at::Tensor> forward(const Call& c, bool stats) {
@@ -598,10 +552,10 @@ std::vector<at::Tensor> forward(const Call& c, bool stats) {
           launch(attend_few_kernel<T, ED, false>, blocks, 256, lds, p,
                  stream);
       } else if constexpr (sizeof(T) == 2 && ED <= 64) {
-        if (twice) launch_attend<T, ED, 2>(p, stream);
-        else launch_attend<T, ED, 1>(p, stream);
+        if (twice) launch_attend<T, ED, 2>(p, blocks, stream);
+        else launch_attend<T, ED, 1>(p, blocks, stream);
       } else {
-        launch_attend<T, ED, 1>(p, stream);
+        launch_attend<T, ED, 1>(p, blocks, stream);
       }
     });
     if (p.splits > 1)
@@ -700,11 +654,11 @@ Call checked(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     }
     TORCH_CHECK_VALUE(key_step >= 1, "cross_attention: key_step has to be 1 "
                       "or more, got ", key_step);
-    const long limit = 1L << 30;
+    const long limit = 1L << 27;
     TORCH_CHECK_VALUE(key_step < limit && key_step * (Lk + 128) < limit &&
                           query_start > -limit && query_start < limit &&
                           std::abs(query_start) + Lq + 256 < limit,
-                      "cross_attention: positions have to stay under 2**30");
+                      "cross_attention: positions have to stay under 2**27");
     c.table = t.contiguous();
   }
   return c;

@@ -179,6 +179,7 @@ void attend_dq_kernel(Args p) {
   }
   float* sums = lines + wave * (2 * far + 1) + far;
 
+  const Line bias_line(line, far);
   f32x16 acc[DB] = {};
   const float scale = p.scale * kLog2e;
   const T* kb = (const T*)p.k + n * p.kn + hk * p.kh;
@@ -229,11 +230,13 @@ void attend_dq_kernel(Args p) {
                        (lane & 31);
         float ds[16];
         if (LINED && side == 0) {
+          const int a0 = bias_line.at(d0);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int d = d0 + M::seq(j, 0) * p.bias.key_step;
-            ds[j] = fmaf(c[j], scale, line[max(-far, min(d, far))]) - lse;
-          }
+          for (int j = 0; j < 16; ++j)
+            ds[j] = fmaf(c[j], scale,
+                         bias_line.get(a0 + 4 * M::seq(j, 0) *
+                                                p.bias.key_step)) -
+                    lse;
         } else {
           const float off =
               (!LINED ? 0.0f : side > 0 ? behind : before) - lse;

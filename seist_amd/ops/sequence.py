@@ -128,9 +128,9 @@ def _check_cross_attention(q, k, v, kv_lengths, bias_table, scale, key_step,
                         f"{bias_table.dtype} on {bias_table.device}")
         if key_step < 1:
             _refuse(op, f"key_step has to be 1 or more, got {key_step}")
-        if key_step * (k.size(3) + 128) >= 2 ** 30 \
-                or abs(query_start) + q.size(3) + 256 >= 2 ** 30:
-            _refuse(op, "positions have to stay under 2**30")
+        if key_step * (k.size(3) + 128) >= 2 ** 27 \
+                or abs(query_start) + q.size(3) + 256 >= 2 ** 27:
+            _refuse(op, "positions have to stay under 2**27")
 
 
 def _cross_attention_plain(q, k, v, lengths, table, scale, key_step,

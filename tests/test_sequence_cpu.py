@@ -108,8 +108,8 @@ def test_buckets(buckets, far):
     (dict(bias_table=torch.zeros(2, 8), max_distance=2), "max_distance"),
     (dict(bias_table=torch.zeros(2, 8), max_distance=1025), "max_distance"),
     (dict(bias_table=torch.zeros(2, 8), key_step=0), "key_step"),
-    (dict(bias_table=torch.zeros(2, 8), key_step=2 ** 29), "2\\*\\*30"),
-    (dict(bias_table=torch.zeros(2, 8), query_start=-2 ** 30), "2\\*\\*30"),
+    (dict(bias_table=torch.zeros(2, 8), key_step=2 ** 29), "2\\*\\*27"),
+    (dict(bias_table=torch.zeros(2, 8), query_start=-2 ** 30), "2\\*\\*27"),
 ])
 def test_attention_refuses(change, word):
     args = dict(q=torch.zeros(1, 2, 4, 2), k=torch.zeros(1, 2, 4, 3),
