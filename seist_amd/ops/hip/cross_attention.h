@@ -407,7 +407,7 @@ inline void launch(K kernel, long blocks, int threads, size_t lds, const Args& p
 template <typename T, int ED>
 constexpr int tile_positions() {
   constexpr int bytes = ED * sizeof(T);
-  return bytes >= 512 ? 32 : bytes > 64 ? 64 : 128;
+  return bytes > 256 ? 32 : bytes > 64 ? 64 : 128;
 }
 
 template <typename F>
@@ -415,6 +415,7 @@ inline void with_depth(int E, F f) {
   if (E <= 16) f(std::integral_constant<int, 16>{});
   else if (E <= 32) f(std::integral_constant<int, 32>{});
   else if (E <= 64) f(std::integral_constant<int, 64>{});
+  else if (E <= 96) f(std::integral_constant<int, 96>{});
   else f(std::integral_constant<int, 128>{});
 }
 

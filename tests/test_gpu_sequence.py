@@ -56,6 +56,8 @@ def _check_attention(q, k, v, do, table, lens=None, **more):
     (1, 6, 1, 64, 5, 1000),     # 30 rows of six heads in one tile, split keys
     (1, 2, 1, 72, 130, 129),    # past a workgroup's rows, odd channels
     (1, 2, 2, 128, 200, 77),    # the widest heads
+    (1, 2, 1, 96, 150, 300),
+    (1, 1, 1, 97, 70, 200),
     (1, 1, 1, 33, 1, 2500),     # a long split of the keys
     (1, 1, 1, 17, 2500, 3),     # few keys: a long split of the queries
     (3, 33, 1, 8, 1, 40),       # 33 heads share a key head
@@ -137,6 +139,60 @@ def test_attention_views(dtype):
             for t in (q, k, v, do)]
     _check_attention(*last, None)
     _check_attention(q, k, v, do[:, :, :, :1].expand(2, 3, 16, 65), None)
+
+
+REFUSED_ATTENTION = [
+    (dict(q=(1, 3, 4, 2)), "share"),
+    (dict(q=(1, 2, 4)), "needed"),
+    (dict(v=(1, 2, 4, 4)), "needed"),
+    (dict(q=(1, 2, 5, 2)), "needed"),
+    (dict(q=(1, 2, 129, 2), k=(1, 2, 129, 3), v=(1, 2, 129, 3)), "channels"),
+    (dict(q=(1, 2, 0, 2), k=(1, 2, 0, 3), v=(1, 2, 0, 3)), "channels"),
+    (dict(k=(1, 0, 4, 3), v=(1, 0, 4, 3)), "share"),
+    (dict(scale=0.0), "scale"),
+    (dict(scale=-1.0), "scale"),
+    (dict(scale=math.inf), "scale"),
+    (dict(scale=math.nan), "scale"),
+    (dict(kv_lengths=torch.zeros(2, dtype=torch.int32)), "kv_lengths"),
+    (dict(kv_lengths=torch.zeros(1)), "kv_lengths"),
+    (dict(bias_table=(1, 8)), "bias_table"),
+    (dict(bias_table=(2, 8, 1)), "bias_table"),
+    (dict(bias_table=(2, 7)), "buckets"),
+    (dict(bias_table=(2, 2)), "buckets"),
+    (dict(bias_table=(2, 66)), "buckets"),
+    (dict(bias_table=(2, 8), max_distance=2), "max_distance"),
+    (dict(bias_table=(2, 8), max_distance=1025), "max_distance"),
+    (dict(bias_table=(2, 8), key_step=0), "key_step"),
+    (dict(bias_table=(2, 8), key_step=2 ** 26), "positions"),
+    (dict(bias_table=(2, 8), query_start=-2 ** 27), "positions"),
+    (dict(bias_table=(2, 8), query_start=2 ** 62), "positions"),
+]
+
+
+@pytest.mark.parametrize("change,word", REFUSED_ATTENTION)
+def test_attention_refuses(change, word):
+    args = dict(q=(1, 2, 4, 2), k=(1, 2, 4, 3), v=(1, 2, 4, 3))
+    args.update(change)
+    for name, a in args.items():
+        if isinstance(a, tuple):
+            args[name] = torch.zeros(a, device=DEV)
+        elif isinstance(a, torch.Tensor):
+            args[name] = a.to(DEV)
+    with pytest.raises(ValueError, match=word):
+        ops.cross_attention(**args)
+
+
+def test_attention_refuses_types_and_places():
+    q, k, v, do, table = _attention_inputs(1, 2, 2, 8, 5, 4, 8, FP32)
+    for args in ((q.half(), k.half(), v.half()), (q, k.bfloat16(), v),
+                 (q, k.cpu(), v), (q, k, v, None, table.bfloat16()),
+                 (q, k, v, torch.zeros(1, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            ops.cross_attention(*args)
+    q.requires_grad_()
+    out = ops.cross_attention(q, k, v)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(out, q, do, create_graph=True)
 
 
 def test_attention_empty():
@@ -333,6 +389,38 @@ def test_scan_one_gradient_alone():
                                    dh if through == 0 else None,
                                    ds if through == 1 else None)
             ref.assert_within(got, want["dx"], bound["dx"], "dx")
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(x=(2, 3)), "needed"),
+    (dict(gate=(2, 3, 5)), "needed"),
+    (dict(x=(2, 3, 0), gate=(2, 3, 0)), "at least 1"),
+    (dict(state=(2, 4)), "state"),
+    (dict(state=(2, 3, 1)), "state"),
+    (dict(lengths=torch.zeros(3, dtype=torch.int32)), "lengths"),
+    (dict(lengths=torch.zeros(2)), "lengths"),
+])
+def test_scan_refuses(change, word):
+    args = dict(x=(2, 3, 4), gate=(2, 3, 4))
+    args.update(change)
+    for name, a in args.items():
+        args[name] = torch.zeros(a, device=DEV) if isinstance(a, tuple) \
+            else a.to(DEV)
+    with pytest.raises(ValueError, match=word):
+        ops.gated_scan(**args)
+
+
+def test_scan_refuses_types_and_places():
+    x, gate, state, dh, _ = _scan_inputs(2, 3, 4, FP32)
+    for args in ((x.half(), gate.half()), (x, gate.bfloat16()),
+                 (x, gate.cpu()), (x, gate, state.bfloat16()),
+                 (x, gate, state.cpu())):
+        with pytest.raises(ValueError):
+            ops.gated_scan(*args)
+    x.requires_grad_()
+    h, _ = ops.gated_scan(x, gate)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(h, x, dh, create_graph=True)
 
 
 def test_scan_empty():
