@@ -37,6 +37,7 @@ struct Args {
   void *out, *dk, *dv;
   float* lse;      // (N, H, Lq), log2; +inf where a query has no key
   float* delta;    // (N, H, Lq)
+  float* deltas;   // (splits, 2, N, H, Lq), shares of sum p dp and of sum p
   float* part;     // split results, fp32
   float* stat;     // split maxima and sums
   float* dbias;    // (N * splits, H, tiles of 128 rows, buckets)
@@ -274,6 +275,42 @@ __device__ __forceinline__ void own_columns(
   for (int kk = 0; kk < ED / Mma<T>::kDepth; ++kk)
     op[kk] = Mma<T>::template first<Columns<T, ED>::kStride, false>(lds, kk,
                                                                     0);
+}
+
+// A wave's 32 columns of channels, as the second product leaves them, out to
+// memory: `to` is channel 0 of the first column, `count` columns are there.
+// By way of `lds`, which is this wave's, so that 16 bytes go out at a time
+// and not an element (bf16: 64 lanes then write 1 KB and not 128 bytes).
+template <typename T, int ED, int DB>
+__device__ __forceinline__ void put_columns(T* lds, const f32x16 (&acc)[DB],
+                                            float by, T* to, long stride,
+                                            int E, int count) {
+  using C = Columns<T, ED>;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  wave_fence();
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int e = 32 * d + 8 * (j / 4) + 4 * h + j % 4;
+      if (ED % 32 == 0 || e < ED)
+        lds[e * C::kStride + (lane & 31)] = (T)(acc[d][j] * by);
+    }
+  wave_fence();
+#pragma unroll
+  for (int o = 0; o < C::kOwn; ++o) {
+    const int e = C::row_of(lane, o), col = C::col_of(lane, o);
+    if (e >= E) continue;
+    const T* from = lds + e * C::kStride + col;
+    T* at = to + e * stride + col;
+    if (col + C::kVec <= count) {
+      const typename C::Chunk c = *(const typename C::Chunk*)from;
+      __builtin_memcpy(at, &c, sizeof(c));
+    } else {
+#pragma unroll 1
+      for (int j = 0; col + j < count; ++j) at[j] = from[j];
+    }
+  }
 }
 
 // over the two lanes that a column has, one in each half of the wave

@@ -223,13 +223,16 @@ attend_kernel(Args p) {
     }
   }
 
+  __syncthreads();  // the results pass through where the tiles were
+  if (first - g * p.pad >= p.Lq || first >= p.G * p.pad) return;
 #pragma unroll
   for (int o = 0; o < QB; ++o) {
     const float all = both_sum(sum[o]);
     const int i = i0 + 32 * o;
-    if (i >= p.Lq || first >= p.G * p.pad) continue;
+    const long to = (long)n * p.H + head;
     if (p.splits > 1) {
       const int rows = p.G * p.pad, row = first + 32 * o + (lane & 31);
+      if (i >= p.Lq) continue;
       const long at = (long)split * p.N * p.Hkv + nh;
       float* out = p.part + at * p.E * rows + row;
 #pragma unroll
@@ -246,17 +249,12 @@ attend_kernel(Args p) {
       continue;
     }
     const float inv = all > 0.0f ? 1.0f / all : all;  // 0 stays, NaN stays
-    T* out = (T*)p.out + ((long)n * p.H + head) * p.E * p.Lq + i;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int e = 32 * d + 8 * (j / 4) + 4 * h + j % 4;
-        if (e < p.E) out[(long)e * p.Lq] = (T)(acc[o][d][j] * inv);
-      }
-    if (p.lse && h == 0)
-      p.lse[((long)n * p.H + head) * p.Lq + i] =
-          all == 0.0f ? INFINITY : most[o] + log2f(all);
+    const int from = first - g * p.pad + 32 * o;
+    put_columns<T, ED>(
+        (T*)shared + wave * (Columns<T, ED>::kBytes / sizeof(T)), acc[o], inv,
+        (T*)p.out + to * p.E * p.Lq + from, p.Lq, p.E, p.Lq - from);
+    if (p.lse && h == 0 && i < p.Lq)
+      p.lse[to * p.Lq + i] = all == 0.0f ? INFINITY : most[o] + log2f(all);
   }
 }
 

@@ -105,19 +105,29 @@ __device__ __forceinline__ void add_diagonals(const Bias& b,
   }
 }
 
-// As the forward kernel, a wave has 32 queries along its lanes. TABLE: the
-// gradient of the bias, too. Its entries sum ds over many pairs, and ds of a
-// query sums to zero over its keys; a delta made from the rounded output
-// would leave a remainder there that outgrows the entries, so bf16 walks the
-// keys once more beforehand for the delta that belongs to these p and dp.
-template <typename T, int ED, int POS, bool LINED, bool TABLE>
+// As the forward kernel, a wave has 32 queries along its lanes. What it is to
+// find:
+// DQ     dq, with delta from the output
+// DELTA  delta alone, from these p and dp
+// TABLE  dq and the gradient of the bias, with a given delta.
+// delta is the mean of dp under p. An entry of the bias sums ds over many
+// pairs, and ds of a query sums to zero over its keys; a delta made from the
+// output, which is rounded and whose p was, would leave a remainder there that
+// outgrows the entries. So where the bias has a gradient, the keys are walked
+// once more beforehand, and the mean is over what the same weights sum to: a
+// logarithm of 13 has steps of 1e-6, and p with it.
+// Where a query has 32 keys at most, its p and dp are in registers at once and
+// delta is theirs too: with few keys the output is no smaller than a value,
+// and so is its rounding.
+enum Find { DQ, DELTA, TABLE };
+
+template <typename T, int ED, int POS, bool LINED, Find FIND>
 __global__ __launch_bounds__(
     256, ED * (LINED ? 2 : 1) * (sizeof(T) == 2 ? 2 : 8) <= 256 ? 2 : 1)
 void attend_dq_kernel(Args p) {
   using M = Mma<T>;
   using Staged = Tile<T, ED, POS, 256>;
   constexpr int DB = (ED + 31) / 32;
-  constexpr bool TWICE = TABLE && sizeof(T) == 2;
   extern __shared__ char shared[];
 
   const Place place(p, p.tiles * p.splits);
@@ -146,10 +156,26 @@ void attend_dq_kernel(Args p) {
                      p.E, i0, p.Lq);
   own_columns<T, ED>(go, own, (const T*)p.dout + n * p.dn + head * p.dh,
                      p.de, p.E, i0, p.Lq);
+  const long rows = (long)p.N * p.H * p.Lq;
   const long stat = ((long)n * p.H + head) * p.Lq + i;
-  const float lse = live ? p.lse[stat] : INFINITY;
+  // Where the bias has a gradient, the weights are 2^up times p, so that their
+  // logarithms are near zero and not near log2 of the keys' number: a rounding
+  // there is an error of each p that the last buckets sum up.
+  const int up = FIND == DQ ? 0 : 31 - __clz(total | 1);
+  const float down = __builtin_ldexpf(1.0f, -up);
+  const float lse = live ? p.lse[stat] - up : INFINITY;
   float delta = 0.0f;
-  if (!TWICE) {
+  float weight = 0.0f;  // what the weights sum to
+  const bool few = FIND == DQ && total <= 32;
+  if (FIND == TABLE && live) {
+    for (int s = 0; s < p.splits; ++s) {
+      const float* of = p.deltas + 2 * s * rows + stat;
+      delta += of[0];
+      weight += of[rows];
+    }
+    if (weight != 0.0f) delta /= weight;
+  }
+  if (FIND == DQ && !few) {
     typename M::Op o[ED / M::kDepth];
     own_columns<T, ED>(o, own,
                        (const T*)p.o + ((long)n * p.H + head) * p.E * p.Lq,
@@ -174,7 +200,7 @@ void attend_dq_kernel(Args p) {
     spread_bias<T, false>(p.bias, head, line, tid, 256);
     before = bias_of<T>(p.bias, head, -far);
     behind = bias_of<T>(p.bias, head, far);
-    if (TABLE)
+    if (FIND == TABLE)
       for (int d = tid; d < 4 * (2 * far + 1); d += 256) lines[d] = 0.0f;
   }
   float* sums = lines + wave * (2 * far + 1) + far;
@@ -191,115 +217,137 @@ void attend_dq_kernel(Args p) {
     for (int b = 0; b < 4; ++b)
       Staged::blank((T*)(shared + b * Staged::kBytes), p.E, tid);
 
-#pragma unroll 1
-  for (int walk = TWICE ? 0 : 1; walk < 2; ++walk) {
-    if (begin < end) {
-      ks.load(kb, begin, end, tid);
-      vs.load(vb, begin, end, tid);
-    }
-    if (TWICE) __syncthreads();  // the other walk's last tile
-    int buf = 0;
-    for (int at = begin; at < end; at += POS, buf ^= 1) {
-      T* kt = (T*)(shared + 2 * buf * Staged::kBytes);
-      T* vt = (T*)(shared + (2 * buf + 1) * Staged::kBytes);
-      ks.store(kt, p.E, tid);
-      vs.store(vt, p.E, tid);
-      __syncthreads();
-      if (at + POS < end) {
-        ks.load(kb, at + POS, end, tid);
-        vs.load(vb, at + POS, end, tid);
-      }
-      if (i0 >= p.Lq) continue;  // no query of this wave's
-#pragma unroll 1
-      for (int col = 0; col < POS && at + col < end; col += 32) {
-        const int key0 = at + col;
-        f32x16 c = {}, dp = {};
-#pragma unroll
-        for (int kk = 0; kk < ED / M::kDepth; ++kk) {
-          c = M::mul(M::template first<Staged::kStride>(kt, kk, col), q[kk],
-                     c);
-          dp = M::mul(M::template first<Staged::kStride>(vt, kk, col),
-                      go[kk], dp);
-        }
-        int side = 2;
-        if (LINED)
-          side = beyond(p.bias, key0 * p.bias.key_step - (from + 31),
-                        (key0 + 31) * p.bias.key_step - from);
-        // the lane's own part of a distance; the rest is the wave's
-        const int d0 = (key0 + M::seq(0, h)) * p.bias.key_step - from -
-                       (lane & 31);
-        float ds[16];
-        if (LINED && side == 0) {
-          const int a0 = bias_line.at(d0);
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            ds[j] = fmaf(c[j], scale,
-                         bias_line.get(a0 + 4 * M::seq(j, 0) *
-                                                p.bias.key_step)) -
-                    lse;
-        } else {
-          const float off =
-              (!LINED ? 0.0f : side > 0 ? behind : before) - lse;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) ds[j] = fmaf(c[j], scale, off);
-        }
-        if (key0 + 32 > end) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (key0 + M::seq(j, h) >= end) ds[j] = -INFINITY;
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) ds[j] = __builtin_amdgcn_exp2f(ds[j]);
-        if (TWICE && walk == 0) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) delta = fmaf(ds[j], dp[j], delta);
-          continue;
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) ds[j] *= dp[j] - delta;
-        if (TABLE && side == 0) {
-          add_diagonals<T>(p.bias, ds, diagonals, sums,
-                           key0 * p.bias.key_step - from, ds_before,
-                           ds_behind);
-        } else if (TABLE) {
-          float all = 0.0f;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) all += ds[j];
-          if (side > 0) ds_behind += all;
-          else ds_before += all;
-        }
-        typename M::Right pr;
-        M::right(pr, ds);
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-          acc[d] = M::mul(
-              M::template second<Staged::kStride, ED>(kt, 32 * d, col), pr,
-              acc[d]);
-      }
-    }
-    if (TWICE && walk == 0) delta = both_sum(delta);
+  if (begin < end) {
+    ks.load(kb, begin, end, tid);
+    vs.load(vb, begin, end, tid);
   }
-  const int rows = p.G * p.pad;
-  if (TABLE)  // a workgroup's rows are one head's, and there are some
+  int buf = 0;
+  for (int at = begin; at < end; at += POS, buf ^= 1) {
+    T* kt = (T*)(shared + 2 * buf * Staged::kBytes);
+    T* vt = (T*)(shared + (2 * buf + 1) * Staged::kBytes);
+    ks.store(kt, p.E, tid);
+    vs.store(vt, p.E, tid);
+    __syncthreads();
+    if (at + POS < end) {
+      ks.load(kb, at + POS, end, tid);
+      vs.load(vb, at + POS, end, tid);
+    }
+    if (i0 >= p.Lq) continue;  // no query of this wave's
+#pragma unroll 1
+    for (int col = 0; col < POS && at + col < end; col += 32) {
+      const int key0 = at + col;
+      f32x16 c = {}, dp = {};
+#pragma unroll
+      for (int kk = 0; kk < ED / M::kDepth; ++kk) {
+        c = M::mul(M::template first<Staged::kStride>(kt, kk, col), q[kk],
+                   c);
+        dp = M::mul(M::template first<Staged::kStride>(vt, kk, col),
+                    go[kk], dp);
+      }
+      int side = 2;
+      if (LINED)
+        side = beyond(p.bias, key0 * p.bias.key_step - (from + 31),
+                      (key0 + 31) * p.bias.key_step - from);
+      // the lane's own part of a distance; the rest is the wave's
+      const int d0 = (key0 + M::seq(0, h)) * p.bias.key_step - from -
+                     (lane & 31);
+      float ds[16];
+      if (LINED && side == 0) {
+        const int a0 = bias_line.at(d0);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          ds[j] = fmaf(c[j], scale,
+                       bias_line.get(a0 + 4 * M::seq(j, 0) *
+                                              p.bias.key_step)) -
+                  lse;
+      } else {
+        const float off =
+            (!LINED ? 0.0f : side > 0 ? behind : before) - lse;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) ds[j] = fmaf(c[j], scale, off);
+      }
+      if (key0 + 32 > end) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (key0 + M::seq(j, h) >= end) ds[j] = -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) ds[j] = __builtin_amdgcn_exp2f(ds[j]);
+      if (FIND == DELTA) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          delta = fmaf(ds[j], dp[j], delta);
+          weight += ds[j];
+        }
+        continue;
+      }
+      if (few) {
+        float all = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          delta = fmaf(ds[j], dp[j], delta);
+          all += ds[j];
+        }
+        all = both_sum(all);
+        delta = both_sum(delta);
+        if (all != 0.0f) delta /= all;
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        ds[j] *= FIND == DQ ? dp[j] - delta : fmaf(dp[j], down, -delta * down);
+      if (FIND == TABLE && side == 0) {
+        add_diagonals<T>(p.bias, ds, diagonals, sums,
+                         key0 * p.bias.key_step - from, ds_before,
+                         ds_behind);
+      } else if (FIND == TABLE) {
+        float all = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) all += ds[j];
+        if (side > 0) ds_behind += all;
+        else ds_before += all;
+      }
+      typename M::Right pr;
+      M::right(pr, ds);
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+        acc[d] = M::mul(
+            M::template second<Staged::kStride, ED>(kt, 32 * d, col), pr,
+            acc[d]);
+    }
+  }
+  if (FIND == DELTA) {
+    delta = both_sum(delta);
+    weight = both_sum(weight);
+    if (first < p.G * p.pad && live && h == 0) {
+      float* to = p.deltas + 2 * split * rows + stat;
+      to[0] = delta;
+      to[rows] = weight;
+    }
+    return;
+  }
+  if (FIND == TABLE)  // a workgroup's rows are one head's, and there are some
     fold_table(p.bias, lines, ds_before, ds_behind, ends,
                p.dbias + (((long)(n * p.splits + split) * p.H + head) *
                               (p.pad / 128) + i0 / 128) * p.bias.buckets);
-  if (first >= rows || !live) return;
-  if (split == 0 && h == 0) p.delta[stat] = delta;
-  const long to = ((long)n * p.H + head) * p.E * p.Lq + i;
+  __syncthreads();  // the results pass through where the tiles were
+  if (first >= p.G * p.pad || i0 >= p.Lq) return;
+  if (live && split == 0 && h == 0) p.delta[stat] = delta;
+  const long to = ((long)n * p.H + head) * p.E * p.Lq + i0;
+  if (p.splits > 1) {
+    if (!live) return;
+    float* out = p.part + (long)split * p.N * p.H * p.E * p.Lq + to +
+                 (lane & 31);
 #pragma unroll
-  for (int d = 0; d < DB; ++d)
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int e = 32 * d + 8 * (j / 4) + 4 * h + j % 4;
-      if (e >= p.E) continue;
-      const float v = acc[d][j] * p.scale;
-      if (p.splits > 1)
-        p.part[(long)split * p.N * p.H * p.E * p.Lq + to +
-               (long)e * p.Lq] = v;
-      else
-        ((T*)p.out)[to + (long)e * p.Lq] = (T)v;
-    }
+      for (int j = 0; j < 16; ++j) {
+        const int e = 32 * d + 8 * (j / 4) + 4 * h + j % 4;
+        if (e < p.E) out[(long)e * p.Lq] = acc[d][j] * p.scale;
+      }
+    return;
+  }
+  put_columns<T, ED>(own, acc, p.scale, (T*)p.out + to, p.Lq, p.E,
+                     p.Lq - i0);
 }
 
 // --- backward: dk, dv --------------------------------------------------------
@@ -432,27 +480,35 @@ struct Walk {
     __syncthreads();
     if (row + POS < end) fetch(row + POS);
   }
-  // a wave's columns of dk or dv
+  // A wave's columns of dk or dv, by way of its own part of the LDS: all
+  // waves have to be past the tiles.
   template <int DB>
-  __device__ __forceinline__ void store(const f32x16 (&acc)[DB], T* out,
-                                        int half, int key, float by) const {
-    if (key >= p.Lk) return;
+  __device__ __forceinline__ void store(f32x16 (&acc)[DB], T* out, int half,
+                                        int key0, float by) const {
+    if (key0 >= p.Lk) return;
+    const int lane = tid & 63, h = lane >> 5, key = key0 + (lane & 31);
     // a key that does not count has gone through with k = v = 0: its column
     // holds numbers of no meaning
-    const bool live = key < total;
-    const int h = (tid & 63) >> 5;
-    const long to = (long)nh * p.E * p.Lk + key;
+    if (key >= total) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
+    }
+    const long to = (long)nh * p.E * p.Lk;
+    if (p.splits == 1) {
+      put_columns<T, ED>(
+          (T*)shared + wave * (Columns<T, ED>::kBytes / sizeof(T)), acc, by,
+          out + to + key0, p.Lk, p.E, p.Lk - key0);
+      return;
+    }
+    if (key >= p.Lk) return;
     float* part = p.part + ((long)half * p.splits + split) * p.N * p.Hkv *
-                               p.E * p.Lk;
+                               p.E * p.Lk + to + key;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int e = 32 * d + 8 * (j / 4) + 4 * h + j % 4;
-        if (e >= p.E) continue;
-        const float v = live ? acc[d][j] * by : 0.0f;
-        if (p.splits > 1) part[to + (long)e * p.Lk] = v;
-        else out[to + (long)e * p.Lk] = (T)v;
+        if (e < p.E) part[(long)e * p.Lk] = acc[d][j] * by;
       }
   }
 };
@@ -528,9 +584,9 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(Args p) {
       }
     }
   }
-  const int key = key0 + (threadIdx.x & 31);
-  w.template store<DB>(dk, (T*)p.dk, 0, key, p.scale);
-  w.template store<DB>(dv, (T*)p.dv, 1, key, 1.0f);
+  __syncthreads();
+  w.template store<DB>(dk, (T*)p.dk, 0, key0, p.scale);
+  w.template store<DB>(dv, (T*)p.dv, 1, key0, 1.0f);
 }
 
 // For deep heads a wave's k, v, dk and dv alone are 192 registers, and a SIMD
@@ -627,9 +683,9 @@ __global__ __launch_bounds__(512, 2) void attend_dkv_pair_kernel(Args p) {
                         r, acc[d]);
     }
   }
-  const int key = key0 + (lane & 31);
-  w.template store<DB>(acc, second ? (T*)p.dk : (T*)p.dv, second ? 0 : 1, key,
-                       second ? p.scale : 1.0f);
+  __syncthreads();
+  w.template store<DB>(acc, second ? (T*)p.dk : (T*)p.dv, second ? 0 : 1,
+                       key0, second ? p.scale : 1.0f);
 }
 
 // out[i] = sum of `splits` runs of `count`
@@ -707,16 +763,15 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
   // with a bias, a workgroup's rows are one head's
   p.pad = round_up(p.Lq, p.bias.table ? 128 : 32);
   p.tiles = sa::ceil_div((long)p.G * p.pad, 128);
-  // no cut where delta comes from a first walk over all keys
-  const bool twice = table && c.q.scalar_type() == at::kBFloat16;
-  p.splits =
-      cut(twice ? 1L << 40 : pairs * p.tiles, p.Lk, 128, &p.per_split);
-  at::Tensor part, sums;
+  p.splits = cut(pairs * p.tiles, p.Lk, 128, &p.per_split);
+  at::Tensor part, sums, deltas;
   if (p.splits > 1) {
     part = at::empty({p.splits, c.q.numel()}, f32);
     p.part = part.data_ptr<float>();
   }
   if (table) {
+    deltas = at::empty({p.splits, 2, p.N, p.H, p.Lq}, f32);
+    p.deltas = deltas.data_ptr<float>();
     sums = at::empty({p.N * p.splits, p.H, p.pad / 128, p.bias.buckets}, f32);
     p.dbias = sums.data_ptr<float>();
   }
@@ -727,15 +782,19 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
       constexpr int ED = decltype(depth)::value;
       constexpr int POS = tile_positions<T, ED>();
       const long blocks = pairs * p.splits * p.tiles;
-      if (table)
-        launch(attend_dq_kernel<T, ED, POS, true, true>, blocks, 256,
-               backward_lds<T, ED>(5 * line + 32 + 4 * 32 * 33 * 4), p, stream);
-      else if (p.bias.table)
-        launch(attend_dq_kernel<T, ED, POS, true, false>, blocks, 256,
+      if (table) {
+        launch(attend_dq_kernel<T, ED, POS, true, DELTA>, blocks, 256,
                backward_lds<T, ED>(line), p, stream);
-      else
-        launch(attend_dq_kernel<T, ED, POS, false, false>, blocks, 256,
+        launch(attend_dq_kernel<T, ED, POS, true, TABLE>, blocks, 256,
+               backward_lds<T, ED>(5 * line + 32 + 4 * 32 * 33 * 4), p,
+               stream);
+      } else if (p.bias.table) {
+        launch(attend_dq_kernel<T, ED, POS, true, DQ>, blocks, 256,
+               backward_lds<T, ED>(line), p, stream);
+      } else {
+        launch(attend_dq_kernel<T, ED, POS, false, DQ>, blocks, 256,
                backward_lds<T, ED>(0), p, stream);
+      }
     });
     if (p.splits > 1) {
       sum_splits_kernel<T><<<sa::ceil_div(c.q.numel(), 256), 256, 0, stream>>>(

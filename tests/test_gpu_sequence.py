@@ -124,6 +124,27 @@ def test_attention_few_query_sums_stay_exact():
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("buckets", [0, 8])
+def test_attention_one_key_has_no_slope(dtype, buckets):
+    # The only key has the weight p = 1 whatever the scores: dq is zero but for
+    # dp - (p dp) / p, off by two roundings to 32 bits, 2 * 2^-24 |dp|, while
+    # dp is at most sum |do| |v|. Twice that covers p's own last bit and the
+    # roundings of ds and dq to the type.
+    q, k, v, do, table = _attention_inputs(2, 2, 1, 48, 70, 40, buckets, dtype)
+    lens = torch.tensor([1, 40], device=DEV)
+    q.requires_grad_()
+    more = {"max_distance": 20} if buckets else {}
+    if buckets:
+        table.requires_grad_()
+    out = ops.cross_attention(q, k, v, lens, table, **more)
+    dq, = torch.autograd.grad(out, [q], do)
+    dp = (do[0].double().abs() * v[0, :, :, :1].double().abs()).sum(1)
+    most = 4 * 2.0 ** -24 * dp[:, None] * k[0, :, :, :1].double().abs()
+    assert (dq[0].double().abs() <= most / math.sqrt(48)).all()
+    assert dq[1].abs().max() > 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_attention_views(dtype):
     """Heads cut out of one projection, steps between samples, and orders
     that need a copy, at odd addresses."""
