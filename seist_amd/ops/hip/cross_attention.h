@@ -427,8 +427,8 @@ struct Place {
 // --- host --------------------------------------------------------------------
 
 template <typename K>
-inline void launch(K kernel, long blocks, int threads, size_t lds, const Args& p,
-            hipStream_t stream) {
+inline void launch(K kernel, long blocks, int threads, size_t lds,
+                   const Args& p, hipStream_t stream) {
   TORCH_CHECK(blocks < (1L << 31), "cross_attention: too many workgroups");
   if (lds > 64 * 1024)
     SA_CHECK_HIP(hipFuncSetAttribute(

@@ -312,6 +312,57 @@ def test_attention_other_stream_and_graph():
         assert all(torch.equal(a, b) for a, b in zip(got[1], eager_other))
 
 
+@pytest.mark.parametrize("lq", [1, 100])
+def test_attention_in_a_long_cache(lq):
+    """Records, and a head's channels, further apart than 32 bits reach: the
+    offsets of the last record's last channel pass 2**32 bytes."""
+    n, e, lk = 2, 128, 300
+    apart, between = 2 ** 31 + 64, 2 ** 24
+    store = torch.empty(apart + e * between, device=DEV, dtype=BF16)
+    k = store.as_strided((n, 1, e, lk), (apart, apart, between, 1), 5)
+    v = store.as_strided((n, 1, e, lk), (apart, apart, between, 1), 1005)
+    q, k0, v0, do, _ = _attention_inputs(n, 2, 1, e, lq, lk, 0, BF16)
+    k.copy_(k0)
+    v.copy_(v0)
+    got = torch.stack([ops.cross_attention(q, k, v),
+                       ops.cross_attention(q, k0, v0)])
+    assert torch.equal(got[0], got[1])
+    leaves = [t.requires_grad_() for t in (q, k0, v0)]
+    want = torch.autograd.grad(ops.cross_attention(*leaves), leaves, do)
+    leaves = [q, k.detach().requires_grad_(), v.detach().requires_grad_()]
+    grads = torch.autograd.grad(ops.cross_attention(*leaves), leaves, do)
+    for a, b in zip(grads, want):
+        assert torch.equal(a, b)
+
+
+def test_attention_deep_heads_in_a_graph():
+    """The largest workgroups, whose LDS has to be asked for, captured, and
+    run on two streams at once."""
+    args = _attention_inputs(2, 2, 1, 128, 200, 700, 32, BF16)
+
+    def step(q, k, v, do, table):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, table)]
+        out = ops.cross_attention(leaves[0], leaves[1], leaves[2], None,
+                                  leaves[3], max_distance=1024)
+        return (out.detach(),) + torch.autograd.grad(out, leaves, do)
+
+    eager = step(*args)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*args)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        graph.replay()
+        both = []
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                both.append(step(*args))
+        torch.cuda.synchronize()
+        for run in [got] + both:
+            assert all(torch.equal(a, b) for a, b in zip(run, eager))
+
+
 def _scan_inputs(n, c, length, dtype, seed=0, shift=1.0):
     g = torch.Generator(device=DEV).manual_seed(seed)
     x, gate, dh = (torch.randn(n, c, length, device=DEV, generator=g)
@@ -473,6 +524,20 @@ def test_scan_against_differences():
         far = (ends[3] - ends[0]) / (4 * step)
         room = abs(far - near) + 2e-4 * dh.norm().item()
         assert abs(near - (grad.double() * way).sum().item()) <= room
+
+
+def test_scan_rows_far_apart():
+    """Rows further apart than 32 bits reach."""
+    apart, length = 2 ** 31 + 8, 5000
+    store = torch.empty(3 * 2 ** 30, device=DEV, dtype=BF16)
+    x, gate = (store.as_strided((2, 2, length), (apart, 8192, 1), at)
+               for at in (3, 40001))
+    near = _scan_inputs(2, 2, length, BF16)
+    x.copy_(near[0])
+    gate.copy_(near[1])
+    for a, b in zip(ops.gated_scan(x, gate),
+                    ops.gated_scan(near[0], near[1])):
+        assert torch.equal(a, b)
 
 
 def test_scan_graph():
