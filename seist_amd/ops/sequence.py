@@ -141,6 +141,11 @@ def _cross_attention_plain(q, k, v, lengths, table, scale, key_step,
     qf = q.float().reshape(N, Hkv, G, E, Lq).transpose(-1, -2)
     kf = k.float().unsqueeze(2)
     vf = v.float().unsqueeze(2)
+    if lengths is not None:
+        hidden = torch.arange(Lk, device=q.device) >= lengths[:, None]
+        # before any product: a gradient of zero times NaN is NaN
+        kf = kf.masked_fill(hidden[:, None, None, None, :], 0.0)
+        vf = vf.masked_fill(hidden[:, None, None, None, :], 0.0)
     s = torch.matmul(qf, kf).reshape(N, H, Lq, Lk) * scale
     if table is not None:
         d = (torch.arange(Lk, device=q.device)[None, :] * key_step
@@ -149,9 +154,7 @@ def _cross_attention_plain(q, k, v, lengths, table, scale, key_step,
             d, table.size(1), max_distance)]
         s = (s + bias).masked_fill(bias <= _OUT, -math.inf)
     if lengths is not None:
-        hidden = torch.arange(Lk, device=q.device) >= lengths[:, None]
         s = s.masked_fill(hidden[:, None, None, :], -math.inf)
-        vf = vf.masked_fill(hidden[:, None, None, None, :], 0.0)
     # a query with no key left has no weights: zeros, and no gradient
     none = (s == -math.inf).all(-1, keepdim=True)
     p = torch.softmax(s.masked_fill(none, 0.0), -1).masked_fill(none, 0.0)

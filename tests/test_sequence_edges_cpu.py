@@ -1,0 +1,35 @@
+"""Calls of the sequence operators at the edges of what their documentation
+allows, on the CPU."""
+
+import math
+
+import pytest
+import torch
+
+import _sequence_ref as ref
+from seist_amd import ops
+
+
+def _inputs(*shapes, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(s, generator=g) for s in shapes]
+
+
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_attention_gradients_do_not_read_masked_places(what):
+    lens = torch.tensor([0, 4, 6])
+    q, k, v, do = _inputs((3, 4, 5, 7), (3, 2, 5, 6), (3, 2, 5, 6),
+                          (3, 4, 5, 7))
+    (table,) = _inputs((4, 8), seed=1)
+    for i, c in enumerate(lens):
+        k[i, :, :, c:], v[i, :, :, c:] = what, what
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    out = ops.cross_attention(q, k, v, lens, table, max_distance=5)
+    grads = torch.autograd.grad(out, leaves, do)
+    want, bound = ref.attention(q, k, v, lens, table, max_distance=5, dout=do)
+    for name, got in zip(("out", "dq", "dk", "dv", "dtable"), (out,) + grads):
+        # the composite also rounds what autograd carries between its steps
+        ref.assert_within(got, want[name], 2 * bound[name], name)
+    assert (grads[0][0] == 0).all()
+    assert (grads[1][1, :, :, 4:] == 0).all()
+    assert (grads[2][1, :, :, 4:] == 0).all()
