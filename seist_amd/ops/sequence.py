@@ -231,13 +231,16 @@ def _check_gated_scan(x, gate, state, lengths):
 
 def _gated_scan_plain(x, gate, state, lengths, reverse):
     N, C, L = x.shape
-    gate = gate.float()
-    a, b = torch.sigmoid(gate), torch.sigmoid(-gate) * x.float()
+    gate, x32 = gate.float(), x.float()
     valid = None
     if lengths is not None:
         valid = torch.arange(L, device=x.device) < lengths[:, None, None]
+        # before any product: a gradient of zero times NaN is NaN
+        gate = torch.where(valid, gate, 0.0)
+        x32 = torch.where(valid, x32, 0.0)
+    a, b = torch.sigmoid(gate), torch.sigmoid(-gate) * x32
+    if valid is not None:
         a = torch.where(valid, a, 1.0)
-        b = torch.where(valid, b, 0.0)
     if reverse:
         a, b = a.flip(-1), b.flip(-1)
     h = x.new_zeros(N, C, dtype=torch.float32) if state is None else state

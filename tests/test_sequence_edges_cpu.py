@@ -33,3 +33,21 @@ def test_attention_gradients_do_not_read_masked_places(what):
     assert (grads[0][0] == 0).all()
     assert (grads[1][1, :, :, 4:] == 0).all()
     assert (grads[2][1, :, :, 4:] == 0).all()
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_scan_gradients_do_not_read_masked_places(what, reverse):
+    lens = torch.tensor([0, 4, 7])
+    x, gate, dh, state, ds = _inputs(*3 * [(3, 2, 7)], *2 * [(3, 2)])
+    for i, c in enumerate(lens):
+        x[i, :, c:], gate[i, :, c:], dh[i, :, c:] = what, what, what
+    leaves = [t.requires_grad_() for t in (x, gate, state)]
+    out = ops.gated_scan(*leaves, lens, reverse)
+    grads = torch.autograd.grad(out, leaves, [dh, ds])
+    want, bound = ref.scan(x, gate, state.detach(), lens, reverse, dh, ds)
+    for name, got in zip(("h", "state", "dx", "dgate", "dstate"),
+                         out + grads):
+        ref.assert_within(got, want[name], bound[name], name)
+    for grad in grads[:2]:
+        assert (grad[0] == 0).all() and (grad[1, :, 4:] == 0).all()
