@@ -80,16 +80,17 @@ def relative_position_buckets(distance: torch.Tensor, num_buckets: int,
     Half of the buckets are for keys at or before the query, half for keys
     after it. Of a half, the first ``num_buckets // 4`` stand for one distance
     each; the rest widen geometrically up to ``max_distance``, and the last
-    holds everything from there on.
+    holds everything from there on. Buckets come in ``distance``'s type.
     """
     _check_buckets("relative_position_buckets", num_buckets, max_distance)
     exact = num_buckets // 4
-    n = distance.abs()
+    # 64 bits hold every threshold, and the size of the lowest 32-bit distance
+    n = (distance if distance.is_floating_point() else distance.long()).abs()
     steps = torch.tensor(_bucket_thresholds(num_buckets, max_distance),
                          dtype=n.dtype, device=n.device)
     at = torch.where(n < exact, n,
                      exact + torch.bucketize(n, steps, right=True).to(n.dtype))
-    return at + (distance > 0).to(n.dtype) * (num_buckets // 2)
+    return (at + (distance > 0) * (num_buckets // 2)).to(distance.dtype)
 
 
 # ---------------------------------------------------------------------------

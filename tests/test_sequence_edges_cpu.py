@@ -51,3 +51,18 @@ def test_scan_gradients_do_not_read_masked_places(what, reverse):
         ref.assert_within(got, want[name], bound[name], name)
     for grad in grads[:2]:
         assert (grad[0] == 0).all() and (grad[1, :, 4:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16,
+                                   torch.int32, torch.int64, torch.float32])
+def test_buckets_of_any_type(dtype):
+    low, high = -2 ** 20, 2 ** 20
+    if not dtype.is_floating_point:
+        ends = torch.iinfo(dtype)
+        low, high = max(ends.min, -2 ** 31), min(ends.max, 2 ** 31 - 1)
+    d = [low, high, high // 2] + list(range(max(low, -120), 121, 7))
+    for buckets, far in ((8, 100), (32, 1024)):
+        got = ops.relative_position_buckets(torch.tensor(d, dtype=dtype),
+                                            buckets, far)
+        assert got.dtype == dtype
+        assert got.tolist() == [ref.bucket(i, buckets, far) for i in d]
