@@ -2,8 +2,8 @@
 length, with a learned position bias, and a gated linear recurrence.
 
 GPU: fused HIP kernels from ``seist_amd._C`` (cross_attention.hip,
-gated_scan.hip). CPU: plain fp32 PyTorch composites with identical
-semantics. Layouts are channels-first: (N, H, E, L) and (N, C, L).
+gated_scan.hip). CPU, and on any device while ``torch.jit`` traces: plain
+fp32 PyTorch composites with identical semantics. Layouts are channels-first: (N, H, E, L) and (N, C, L).
 """
 
 import functools
@@ -26,6 +26,12 @@ _DTYPES = (torch.float32, torch.bfloat16)
 
 def _refuse(op: str, what: str):
     raise ValueError(f"{op}: {what}")
+
+
+def _runs_native(x: torch.Tensor) -> bool:
+    """Whether the kernels run. The tracer sees the extension's allocations and
+    not its launches, so it is given the plain steps, which it records."""
+    return use_native(x) and not torch.jit.is_tracing()
 
 
 def _check_lengths(op: str, name: str, lengths, like: torch.Tensor):
@@ -194,7 +200,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if bias_table is not None and bias_table.dim() == 2:
         _check_buckets("cross_attention", bias_table.size(1), max_distance)
         thresholds = _bucket_thresholds(bias_table.size(1), max_distance)
-    if use_native(q):  # with its own checks, the same as those below
+    if _runs_native(q):  # with its own checks, the same as those below
         return ext().cross_attention(q, k, v, kv_lengths, bias_table, scale,
                                      key_step, query_start, max_distance,
                                      thresholds)
@@ -275,7 +281,7 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor,
     zero, the state stays, and nothing is read into the result. ``reverse``
     runs from the last sample that counts to the first.
     """
-    if use_native(x):  # with its own checks, the same as those below
+    if _runs_native(x):  # with its own checks, the same as those below
         h, last = ext().gated_scan(x, gate, state, lengths, reverse)
         return h, last
     _check_gated_scan(x, gate, state, lengths)

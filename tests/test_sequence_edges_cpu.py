@@ -2,6 +2,7 @@
 allows, on the CPU."""
 
 import math
+import warnings
 
 import pytest
 import torch
@@ -66,3 +67,24 @@ def test_buckets_of_any_type(dtype):
                                             buckets, far)
         assert got.dtype == dtype
         assert got.tolist() == [ref.bucket(i, buckets, far) for i in d]
+
+
+def test_traced_calls_compute_their_own_inputs():
+    q, k, v = _inputs((2, 4, 5, 7), (2, 2, 5, 6), (2, 2, 5, 6))
+    (table,) = _inputs((4, 8), seed=1)
+    x, gate = _inputs((2, 3, 9), (2, 3, 9))
+
+    def attend(q, k, v, table, lens):
+        return ops.cross_attention(q, k, v, lens, table, key_step=2,
+                                   max_distance=5)
+
+    def scan(x, gate, lens):
+        return ops.gated_scan(x, gate, None, lens, True)
+
+    lens = torch.tensor([3, 6])
+    for f, args in ((attend, (q, k, v, table)), (scan, (x, gate))):
+        with warnings.catch_warnings():
+            warnings.simplefilter("ignore")
+            traced = torch.jit.trace(f, (*args, lens), check_trace=False)
+        args = [t * 0.5 - 1 for t in args] + [torch.tensor([6, 0])]
+        torch.testing.assert_close(traced(*args), f(*args), rtol=0, atol=0)
