@@ -585,6 +585,12 @@ std::string shape_of(const at::Tensor& t) {
   return c10::str(t.sizes(), " ", t.scalar_type(), " on ", t.device());
 }
 
+// whether forward mode carries a derivative along with t: the kernels would
+// drop it
+bool has_tangent(const at::Tensor& t) {
+  return t.defined() && t._fw_grad(/*level=*/0).defined();
+}
+
 // What the kernels take for granted. Lengths outside 0..Lk are held to it by
 // the kernels.
 Call checked(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
@@ -606,6 +612,10 @@ Call checked(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
   TORCH_CHECK_VALUE(q.is_cuda() && k.device() == q.device() &&
                         v.device() == q.device(),
                     "cross_attention: q, k and v have to be on one device");
+  TORCH_CHECK(!has_tangent(q) && !has_tangent(k) &&
+                  !has_tangent(v) &&
+                  !(table.has_value() && has_tangent(*table)),
+              "cross_attention: forward-mode derivatives are not available");
   const long H = q.size(1), Hkv = k.size(1), E = q.size(2), Lq = q.size(3),
              Lk = k.size(3);
   TORCH_CHECK_VALUE(Hkv > 0 && H % Hkv == 0, "cross_attention: ", H,
@@ -698,6 +708,8 @@ class CrossAttention : public torch::autograd::Function<CrossAttention> {
       torch::autograd::variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "cross_attention: second derivatives are not available");
+    TORCH_CHECK(!has_tangent(grads[0]),
+                "cross_attention: forward-mode derivatives are not available");
     const auto s = ctx->get_saved_variables();
     const auto where = ctx->saved_data["where"].toIntVector();
     const auto steps = ctx->saved_data["thresholds"].toIntVector();

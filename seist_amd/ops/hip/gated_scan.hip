@@ -714,6 +714,12 @@ at::Tensor along_samples(const at::Tensor& t) {
   return t.stride(2) == 1 ? t : t.contiguous();
 }
 
+// whether forward mode carries a derivative along with t: the kernels would
+// drop it
+bool has_tangent(const at::Tensor& t) {
+  return t.defined() && t._fw_grad(/*level=*/0).defined();
+}
+
 // What the kernels take for granted. Lengths outside 0..L are held to it by
 // the kernels.
 Call checked(const at::Tensor& x, const at::Tensor& gate,
@@ -731,6 +737,9 @@ Call checked(const at::Tensor& x, const at::Tensor& gate,
       type, " and ", gate.scalar_type());
   TORCH_CHECK_VALUE(x.is_cuda() && gate.device() == x.device(),
                     "gated_scan: x and gate have to be on one device");
+  TORCH_CHECK(!has_tangent(x) && !has_tangent(gate) &&
+                  !(state.has_value() && has_tangent(*state)),
+              "gated_scan: forward-mode derivatives are not available");
   TORCH_CHECK_VALUE(x.size(2) < (1L << 30) &&
                         x.size(0) * x.size(1) < (1L << 24),
                     "gated_scan: under 2**30 samples and 2**24 rows are "
@@ -779,6 +788,9 @@ class GatedScan : public torch::autograd::Function<GatedScan> {
       torch::autograd::variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "gated_scan: second derivatives are not available");
+    for (const auto& g : grads)
+      TORCH_CHECK(!has_tangent(g),
+                  "gated_scan: forward-mode derivatives are not available");
     const auto s = ctx->get_saved_variables();
     const Call call = {s[0], s[1], {}, s[2],
                        ctx->saved_data["reverse"].toBool()};

@@ -5,6 +5,7 @@ import warnings
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import _sequence_ref as ref
 from seist_amd import ops
@@ -23,6 +24,49 @@ def _inputs(*shapes, dtype=FP32, seed=0):
 # ---------------------------------------------------------------------------
 # what autograd and the tracer are told
 # ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("at", range(4))
+def test_attention_refuses_forward_mode(at, grad):
+    """A tangent is refused and not dropped, with and without gradients."""
+    args = _inputs((1, 2, 4, 5), (1, 2, 4, 6), (1, 2, 4, 6), (2, 8))
+    tangent = torch.ones_like(args[at])
+    if grad:
+        args = [t.requires_grad_() for t in args]
+    with forward_ad.dual_level():
+        args[at] = forward_ad.make_dual(args[at], tangent)
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(RuntimeError, match="forward-mode"):
+                ops.cross_attention(args[0], args[1], args[2], None, args[3],
+                                    max_distance=5)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("at", range(3))
+def test_scan_refuses_forward_mode(at, grad):
+    args = _inputs((1, 2, 9), (1, 2, 9), (1, 2))
+    tangent = torch.ones_like(args[at])
+    if grad:
+        args = [t.requires_grad_() for t in args]
+    with forward_ad.dual_level():
+        args[at] = forward_ad.make_dual(args[at], tangent)
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(RuntimeError, match="forward-mode"):
+                ops.gated_scan(*args)
+
+
+def test_gradients_refuse_forward_mode():
+    """Forward mode through the backward pass."""
+    q, k, x, gate = (t.requires_grad_() for t in _inputs(
+        (1, 2, 4, 5), (1, 2, 4, 6), (1, 2, 9), (1, 2, 9)))
+    out = ops.cross_attention(q, k, k)
+    h, last = ops.gated_scan(x, gate)
+    with forward_ad.dual_level():
+        for y, leaf in ((out, q), (h, x), (last, x)):
+            dy = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, dy, retain_graph=True)
 
 
 def _traced(f, args):
