@@ -125,7 +125,9 @@ attend_kernel(Args p) {
   const int head = hk * p.G + g;
   const int i0 = first - g * p.pad + (lane & 31);
   float before = 0.0f, behind = 0.0f;
+  float entry = 0.0f;
   if (BIASED) {  // the workgroup's rows are one head's
+    entry = entry_of_lane<T>(p.bias, head);
     spread_bias<T, false>(p.bias, head, line, tid, 256);
     before = bias_of<T>(p.bias, head, -p.bias.max_distance);
     behind = bias_of<T>(p.bias, head, p.bias.max_distance);
@@ -143,6 +145,7 @@ attend_kernel(Args p) {
       Staged::blank((T*)(shared + b * Staged::kBytes), p.E, tid);
 
   const Line bias_line(line, p.bias.max_distance);
+  const bool holes = BIASED && takes_out(entry);
   f32x16 acc[QB][DB] = {};
   float most[QB], sum[QB];
 #pragma unroll
@@ -162,6 +165,15 @@ attend_kernel(Args p) {
 #pragma unroll 1
     for (int col = 0; col < POS && at + col < end; col += STEP) {
       const int key0 = at + col;
+      int side = 2;
+      float add = 0.0f;
+      if (BIASED) {
+        const int from = first - g * p.pad + p.bias.query_start;
+        side = beyond(p.bias, key0 * p.bias.key_step - (from + 32 * QB - 1),
+                      (key0 + STEP - 1) * p.bias.key_step - from);
+        add = side > 0 ? behind : before;
+        if (side != 0 && add == -INFINITY) continue;  // all pairs are out
+      }
       float s[QB][SUBS][16];
 #pragma unroll
       for (int b = 0; b < SUBS; ++b) {
@@ -187,12 +199,6 @@ attend_kernel(Args p) {
 #pragma unroll
               for (int o = 0; o < QB; ++o) s[o][b][j] = -INFINITY;
       }
-      int side = 2;
-      if (BIASED) {
-        const int from = first - g * p.pad + p.bias.query_start;
-        side = beyond(p.bias, key0 * p.bias.key_step - (from + 32 * QB - 1),
-                      (key0 + STEP - 1) * p.bias.key_step - from);
-      }
       if (BIASED && side == 0) {
 #pragma unroll
         for (int o = 0; o < QB; ++o) {
@@ -207,10 +213,19 @@ attend_kernel(Args p) {
                   s[o][b][j], scale,
                   bias_line.get(a0 + 4 * (32 * b + M::seq(j, 0)) *
                                          p.bias.key_step));
+          if (holes) {
+            const int a1 = anew(a0);
+#pragma unroll
+            for (int b = 0; b < SUBS; ++b)
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (bias_line.get(a1 + 4 * (32 * b + M::seq(j, 0)) *
+                                           p.bias.key_step) == -INFINITY)
+                  s[o][b][j] = -INFINITY;
+          }
           weigh<SUBS, DB, true>(s[o], 1.0f, 0.0f, most[o], sum[o], acc[o]);
         }
       } else {
-        const float add = !BIASED ? 0.0f : side > 0 ? behind : before;
 #pragma unroll
         for (int o = 0; o < QB; ++o)
           weigh<SUBS, DB, false>(s[o], scale, add, most[o], sum[o], acc[o]);
@@ -385,13 +400,17 @@ attend_few_kernel(Args p) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int d = (at + M::seq(j, h)) * p.bias.key_step - position;
-        s[0][j] = fmaf(s[0][j], scale,
-                       table[ids[max(-p.bias.max_distance,
-                                     min(d, p.bias.max_distance))]]);
+        const float b = table[ids[max(-p.bias.max_distance,
+                                      min(d, p.bias.max_distance))]];
+        s[0][j] = b == -INFINITY ? b : fmaf(s[0][j], scale, b);
       }
       weigh<1, DB, true>(s, 1.0f, 0.0f, most, sum, acc);
     } else {
       const float add = !BIASED ? 0.0f : side > 0 ? behind : before;
+      if (BIASED && add == -INFINITY) {  // of this lane's head
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[0][j] = 0.0f;
+      }
       weigh<1, DB, false>(s, scale, add, most, sum, acc);
     }
     typename M::Right pr;

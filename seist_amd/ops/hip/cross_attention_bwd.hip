@@ -211,7 +211,9 @@ void attend_dq_kernel(Args p) {
   float* diagonals = ends + 8 + wave * 32 * 33;
   float before = 0.0f, behind = 0.0f;      // bias past the last bucket
   float ds_before = 0.0f, ds_behind = 0.0f;
+  float entry = 0.0f;
   if (LINED) {  // the workgroup's rows are one head's
+    entry = entry_of_lane<T>(p.bias, head);
     spread_bias<T, false>(p.bias, head, line, tid, 256);
     before = bias_of<T>(p.bias, head, -far);
     behind = bias_of<T>(p.bias, head, far);
@@ -221,6 +223,7 @@ void attend_dq_kernel(Args p) {
   float* sums = lines + wave * (2 * far + 1) + far;
 
   const Line bias_line(line, far);
+  const bool holes = LINED && takes_out(entry);
   f32x16 acc[DB] = {};
   f32x16 mean = {};    // sum of p k
   float excess = 0.0f, rounded = 0.0f;  // sums of ds
@@ -253,6 +256,14 @@ void attend_dq_kernel(Args p) {
 #pragma unroll 1
     for (int col = 0; col < POS && at + col < end; col += 32) {
       const int key0 = at + col;
+      int side = 2;
+      float add = 0.0f;
+      if (LINED) {
+        side = beyond(p.bias, key0 * p.bias.key_step - (from + 31),
+                      (key0 + 31) * p.bias.key_step - from);
+        add = side > 0 ? behind : before;
+        if (side != 0 && add == -INFINITY) continue;  // all pairs are out
+      }
       f32x16 c = {}, dp = {};
 #pragma unroll
       for (int kk = 0; kk < ED / M::kDepth; ++kk) {
@@ -261,10 +272,6 @@ void attend_dq_kernel(Args p) {
         dp = M::mul(M::template first<Staged::kStride>(vt, kk, col),
                     go[kk], dp);
       }
-      int side = 2;
-      if (LINED)
-        side = beyond(p.bias, key0 * p.bias.key_step - (from + 31),
-                      (key0 + 31) * p.bias.key_step - from);
       // the lane's own part of a distance; the rest is the wave's
       const int d0 = (key0 + M::seq(0, h)) * p.bias.key_step - from -
                      (lane & 31);
@@ -277,9 +284,17 @@ void attend_dq_kernel(Args p) {
                        bias_line.get(a0 + 4 * M::seq(j, 0) *
                                               p.bias.key_step)) -
                   lse;
+        if (holes) {
+          const int a1 = anew(a0);
+          // a query that is not there is zeros, and NaN by such a key
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (!live || bias_line.get(a1 + 4 * M::seq(j, 0) *
+                                                p.bias.key_step) == -INFINITY)
+              ds[j] = -INFINITY;
+        }
       } else {
-        const float off =
-            (!LINED ? 0.0f : side > 0 ? behind : before) - lse;
+        const float off = add - lse;
 #pragma unroll
         for (int j = 0; j < 16; ++j) ds[j] = fmaf(c[j], scale, off);
       }
@@ -395,15 +410,16 @@ void attend_dq_kernel(Args p) {
 
 // --- backward: dk, dv --------------------------------------------------------
 
-// log2 p of SUBS blocks of 32 queries (rows, from position `from` on) for a
-// wave's 32 keys: scores, bias and the queries' logarithms
+// log2 p of SUBS blocks of 32 queries (rows, from position `from` on, `rows`
+// of them there) for a wave's 32 keys: scores, bias and the queries'
+// logarithms
 template <typename T, int SUBS, bool LINED>
 __device__ __forceinline__ void log_weights(const Args& p,
                                             f32x16 (&c)[SUBS],
                                             const float* lses,
                                             const float* line, float before,
-                                            float behind, int key0,
-                                            int from) {
+                                            float behind, bool holes,
+                                            int key0, int from, int rows) {
   using M = Mma<T>;
   const int lane = threadIdx.x & 63, h = lane >> 5;
   const float scale = p.scale * kLog2e;
@@ -428,8 +444,20 @@ __device__ __forceinline__ void log_weights(const Args& p,
                     l[j & 3];
         }
       }
+      if (holes) {
+        const int d1 = anew(d0);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int d = d1 - M::seq(j, 0);
+          // a query that is not there is zeros, and NaN by such a key
+          if (32 * b + M::seq(j, h) >= rows ||
+              line[line_at<true>(max(-far, min(d, far)))] == -INFINITY)
+            c[b][j] = -INFINITY;
+        }
+      }
     } else {
       const float add = !LINED ? 0.0f : side > 0 ? behind : before;
+      if (LINED && add == -INFINITY) c[b] = f32x16{};
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 l = *(const f32x4*)(lses + 32 * b + M::seq(4 * g, h));
@@ -454,6 +482,7 @@ struct Walk {
   float *stats, *line;  // (2, 2, POS) lse and delta; bias by distance
   Staged qs, os;
   float lse, delta, before, behind;
+  bool holes;  // the head's table takes pairs out
   int lined, buf;
   T *qt, *dt;
   float *lses, *deltas;
@@ -476,6 +505,7 @@ struct Walk {
     lined = -1;
     buf = 0;
     before = behind = 0.0f;
+    holes = false;
     qs.place(p.qe, p.E, tid);
     os.place(p.de, p.E, tid);
   }
@@ -514,9 +544,11 @@ struct Walk {
       const int g = row / p.pad;
       if (g != lined) {  // the next head's
         __syncthreads();
+        const float entry = entry_of_lane<T>(p.bias, hk * p.G + g);
         spread_bias<T, true>(p.bias, hk * p.G + g, line, tid, NT);
         before = bias_of<T>(p.bias, hk * p.G + g, -p.bias.max_distance);
         behind = bias_of<T>(p.bias, hk * p.G + g, p.bias.max_distance);
+        holes = takes_out(entry);
         lined = g;
       }
     }
@@ -602,8 +634,9 @@ __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(Args p) {
                          v[kk], dp[b]);
         }
       log_weights<T, SUBS, LINED>(p, c, w.lses + col, w.line, w.before,
-                                  w.behind, key0,
-                                  p.bias.query_start + i0 + col);
+                                  w.behind, w.holes, key0,
+                                  p.bias.query_start + i0 + col,
+                                  p.Lq - i0 - col);
 #pragma unroll
       for (int b = 0; b < SUBS; ++b) {
         float e[16], ds[16];
@@ -693,7 +726,8 @@ __global__ __launch_bounds__(512, 2) void attend_dkv_pair_kernel(Args p) {
                         c[b]);
       if (!second) {
         log_weights<T, SUBS, LINED>(p, c, w.lses, w.line, w.before, w.behind,
-                                    key0, p.bias.query_start + i0);
+                                    w.holes, key0, p.bias.query_start + i0,
+                                    p.Lq - i0);
 #pragma unroll
         for (int b = 0; b < SUBS; ++b)
 #pragma unroll

@@ -192,7 +192,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     is the number of query positions a key stands for (the pooling ratio of
     pooled keys), ``query_start`` the position of the first query (for queries
     that come one at a time). An entry at or under -1e30, such as -inf or the
-    type's lowest value, takes its pairs out of the softmax.
+    type's lowest value, takes its pairs out of the softmax whatever their
+    scores are, NaN and infinities included. Their weights are zeros, which
+    still meet the values, and in the gradients the keys and queries: only
+    what is behind ``kv_lengths`` may hold anything there.
 
     A query with no key left gives zeros and no gradient.
     """

@@ -1,6 +1,7 @@
 """Calls of the sequence operators at the edges of what their documentation
 allows, on the gfx950 kernels."""
 
+import math
 import warnings
 
 import pytest
@@ -127,3 +128,86 @@ def test_scan_traced(dtype, grad):
         grads = torch.autograd.grad(outs, leaves, [dh, ds])
         for name, got in zip(("dx", "dgate", "dstate"), grads):
             ref.assert_within(got, want[name], bound[name], name)
+
+
+# ---------------------------------------------------------------------------
+# pairs that the table takes out
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("h,hkv,e,lq,lk,far,more", [
+    (2, 2, 16, 70, 100, 6, {}),              # distances past the last bucket
+    (2, 1, 24, 70, 200, 300, {}),            # all of them within it
+    (4, 2, 64, 1, 700, 128, dict(query_start=600)),   # few rows, split keys
+    (4, 2, 8, 3, 90, 20, dict(query_start=40)),
+    (1, 1, 128, 150, 160, 9, {}),            # deep heads, waves in pairs
+    (2, 2, 40, 64, 40, 100, dict(key_step=3)),
+])
+def test_attention_pairs_out_whatever_their_scores(dtype, what, h, hkv, e, lq,
+                                                   lk, far, more):
+    """Keys after every query, with NaN or infinite scores: the results, and
+    all gradients that do not multiply by the keys, are as with finite ones."""
+    q, k, v, do, table = _inputs((1, h, e, lq), (1, hkv, e, lk),
+                                 (1, hkv, e, lk), (1, h, e, lq), (h, 8),
+                                 dtype=dtype)
+    table[:, 4:] = -math.inf
+    want, bound = ref.attention(q, k, v, None, table, max_distance=far,
+                                dout=do, **more)
+    last = more.get("query_start", 0) + lq - 1
+    behind = last // more.get("key_step", 1) + 1
+    assert behind < lk
+    k[..., behind:] = what
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    with torch.no_grad():
+        plain = ops.cross_attention(q, k, v, None, table, max_distance=far,
+                                    **more)
+    out = ops.cross_attention(q, k, v, None, table, max_distance=far, **more)
+    grads = torch.autograd.grad(out, leaves, do)
+    for name, got in zip(("out", "out", "dk", "dv", "dtable"),
+                         (plain, out) + grads[1:]):
+        ref.assert_within(got, want[name], bound[name], name)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("far", [3, 100])
+@pytest.mark.parametrize("e", [16, 128])
+def test_attention_rows_that_leave_a_key_out(dtype, far, e):
+    """A NaN key reaches the queries that have it, and no other."""
+    q, k, v, table = _inputs((1, 2, e, 90), (1, 2, e, 90), (1, 2, e, 90),
+                             (2, 8), dtype=dtype)
+    table[:, 4:] = torch.finfo(dtype).min
+    want, bound = ref.attention(q, k, v, None, table, max_distance=far)
+    k[..., 50] = math.nan
+    out = ops.cross_attention(q, k, v, None, table, max_distance=far)
+    ref.assert_within(out[..., :50], want["out"][..., :50],
+                      bound["out"][..., :50], "out")
+    assert torch.isnan(out[..., 50:]).all()
+
+
+def test_attention_heads_with_and_without_the_pair():
+    """Heads that share a key, of which one has the pair out."""
+    q, k, v, table = _inputs((1, 2, 32, 1), (1, 1, 32, 200), (1, 1, 32, 200),
+                             (2, 8))
+    table[0, 4:] = -math.inf
+    for far in (4, 300):
+        want, bound = ref.attention(q, k, v, None, table, 1, 100, far)
+        bad = k.clone()
+        bad[..., 150] = math.nan
+        out = ops.cross_attention(q, bad, v, None, table, query_start=100,
+                                  max_distance=far)
+        ref.assert_within(out[:, :1], want["out"][:, :1], bound["out"][:, :1],
+                          "out")
+        assert torch.isnan(out[:, 1]).all()
+
+
+def test_attention_no_key_left_and_no_finite_score():
+    """Queries that are NaN and have no key left give zeros."""
+    for lq in (1, 70):
+        q, k, v, table = _inputs((1, 2, 16, lq), (1, 2, 16, 90),
+                                 (1, 2, 16, 90), (2, 8))
+        table[:] = -math.inf
+        q[..., 0] = math.nan
+        out = ops.cross_attention(q, k, v, None, table, max_distance=10)
+        assert (out == 0).all()

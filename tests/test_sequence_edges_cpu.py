@@ -88,3 +88,18 @@ def test_traced_calls_compute_their_own_inputs():
             traced = torch.jit.trace(f, (*args, lens), check_trace=False)
         args = [t * 0.5 - 1 for t in args] + [torch.tensor([6, 0])]
         torch.testing.assert_close(traced(*args), f(*args), rtol=0, atol=0)
+
+
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+def test_attention_pairs_out_whatever_their_scores(what):
+    q, k, v, do = _inputs((1, 2, 4, 7), (1, 2, 4, 12), (1, 2, 4, 12),
+                          (1, 2, 4, 7))
+    (table,) = _inputs((2, 8), seed=1)
+    table[:, 4:] = -math.inf              # no key after the query
+    want, bound = ref.attention(q, k, v, None, table, max_distance=5, dout=do)
+    k[..., 7:] = what
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    out = ops.cross_attention(q, k, v, None, table, max_distance=5)
+    grads = torch.autograd.grad(out, leaves, do)
+    for name, got in zip(("out", "dk", "dv", "dtable"), (out,) + grads[1:]):
+        ref.assert_within(got, want[name], 2 * bound[name], name)
