@@ -596,8 +596,17 @@ std::vector<at::Tensor> forward(const Call& c, bool stats) {
 
 namespace {
 
+// Tile::place reaches a head's channels by 32 bits of bytes, up to the end of
+// a staged tile of 128 positions in the last one, whether or not so many are
+// there.
+bool within_reach(const at::Tensor& t, long stride) {
+  return (stride * (t.size(2) - 1) + 128) * (long)t.element_size() <=
+         (1L << 32);
+}
+
 at::Tensor along_positions(const at::Tensor& t) {
-  return t.stride(3) == 1 ? t : t.contiguous();
+  return t.stride(3) == 1 && within_reach(t, t.stride(2)) ? t
+                                                          : t.contiguous();
 }
 
 std::string shape_of(const at::Tensor& t) {
@@ -652,10 +661,10 @@ Call checked(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                     "cross_attention: scale has to be positive, got ",
                     c.scale);
   for (const auto* t : {&c.q, &c.k, &c.v})
-    TORCH_CHECK_VALUE(
-        t->stride(2) >= 0 && (t->stride(2) * (E - 1) + t->size(3)) *
-                                     (long)t->element_size() < (1L << 32),
-        "cross_attention: a head's channels have to lie within 4 GiB");
+    TORCH_CHECK_VALUE(within_reach(*t, t->stride(2)) &&
+                          within_reach(q, Lq),  // the output, read again
+                      "cross_attention: a head has to fit into 4 GiB, got ",
+                      shape_of(*t));
   if (lengths.has_value()) {
     const auto& l = *lengths;
     TORCH_CHECK_VALUE(
@@ -736,11 +745,7 @@ class CrossAttention : public torch::autograd::Function<CrossAttention> {
                        ctx->saved_data["scale"].toDouble(), where[0],
                        where[1], where[2],
                        std::vector<long>(steps.begin(), steps.end())};
-    at::Tensor dout = along_positions(grads[0]);
-    if (dout.stride(2) < 0 ||
-        (dout.stride(2) * (dout.size(2) - 1) + dout.size(3)) *
-                (long)dout.element_size() >= (1L << 32))
-      dout = dout.contiguous();
+    const at::Tensor dout = along_positions(grads[0]);
     const bool kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     const bool table = call.table.defined() && ctx->needs_input_grad(3);
     auto r = attend::backward(call, s[5], s[6], dout, kv, table);

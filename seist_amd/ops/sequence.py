@@ -180,8 +180,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     q: (N, H, E, Lq); k, v: (N, Hkv, E, Lk) with H a multiple of Hkv, query
     head h reading key head h // (H // Hkv); E up to 128; all bf16 or all
     fp32. Any strides; a copy is made only where the last axis is not
-    contiguous. Returns (N, H, E, Lq) in q's type. ``scale`` defaults to
-    1 / sqrt(E). Differentiable in q, k, v and ``bias_table``.
+    contiguous or a head's channels lie further apart than 4 GiB, which a
+    head has to fit into. Returns (N, H, E, Lq) in q's type. ``scale``
+    defaults to 1 / sqrt(E). Differentiable in q, k, v and ``bias_table``.
 
     ``kv_lengths``: (N,), the keys of each record that count, from 0 to Lk;
     nothing behind them is read into the result, NaN included.

@@ -211,3 +211,47 @@ def test_attention_no_key_left_and_no_finite_score():
         q[..., 0] = math.nan
         out = ops.cross_attention(q, k, v, None, table, max_distance=10)
         assert (out == 0).all()
+
+
+# ---------------------------------------------------------------------------
+# far apart and many
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("lq", [1, 50])
+@pytest.mark.parametrize("short", [128, 127, 60, -8])
+def test_attention_channels_at_the_reach(dtype, lq, short):
+    """A head's channels as far apart as 32 bits of bytes reach, less some
+    positions: short of a staged tile's 128, and past it."""
+    lk, size = 50, torch.finfo(dtype).bits // 8
+    between = 2 ** 32 // size - short
+    store = torch.empty(between + 4096, device=DEV, dtype=dtype)
+    q0, k0, v0, do0 = _inputs((1, 1, 2, lq), (1, 1, 2, lk), (1, 1, 2, lk),
+                              (1, 1, 2, lq), dtype=dtype)
+    far = []
+    for at, t in enumerate((q0, k0, v0, do0)):
+        far.append(store.as_strided(t.shape, (4096, 4096, between, 1),
+                                    1000 * at + 1))
+        far[-1].copy_(t)
+    grads = []
+    for q, k, v, do in ((q0, k0, v0, do0), far):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = ops.cross_attention(*leaves)
+        grads.append((out,) + torch.autograd.grad(out, leaves, do))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@pytest.mark.parametrize("dtype,lq", [(BF16, 2 ** 24 + 2 ** 18),
+                                      (FP32, 2 ** 23 + 2 ** 17)])
+def test_attention_refuses_a_head_of_over_4_gib(dtype, lq):
+    """Queries that overlap in memory, as windows of one record do: they lie
+    close together, their results do not."""
+    (x,) = _inputs((lq + 127,), dtype=dtype)
+    q = x.as_strided((1, 1, 128, lq), (0, 0, 1, 1))
+    k = x[:128 * 5].view(1, 1, 128, 5)
+    with pytest.raises(ValueError, match="4 GiB"):
+        ops.cross_attention(q, k, k)
+    apart = x.as_strided((1, 1, 128, 5), (0, 0, 0, 1))
+    with pytest.raises(ValueError, match="4 GiB"):
+        ops.cross_attention(q, apart, apart)
