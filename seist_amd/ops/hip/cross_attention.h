@@ -453,7 +453,10 @@ struct Place {
 template <typename K>
 inline void launch(K kernel, long blocks, int threads, size_t lds,
                    const Args& p, hipStream_t stream) {
-  TORCH_CHECK(blocks < (1L << 31), "cross_attention: too many workgroups");
+  // a launch has fewer than 2^32 threads
+  TORCH_CHECK_VALUE(blocks * threads < (1L << 32),
+                    "cross_attention: too much work for one launch, ", blocks,
+                    " workgroups of ", threads, "; split the records");
   if (lds > 64 * 1024)
     SA_CHECK_HIP(hipFuncSetAttribute(
         (const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,

@@ -255,3 +255,35 @@ def test_attention_refuses_a_head_of_over_4_gib(dtype, lq):
     apart = x.as_strided((1, 1, 128, 5), (0, 0, 0, 1))
     with pytest.raises(ValueError, match="4 GiB"):
         ops.cross_attention(q, apart, apart)
+
+
+def test_attention_of_the_most_records():
+    """One workgroup a record: as many as a launch holds, and one more."""
+    most = 2 ** 24 - 1
+    q, k, v, do = (t.requires_grad_() for t in _inputs(
+        *4 * [(most, 1, 1, 1)]))
+    out = ops.cross_attention(q, k, v)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), do)
+    # The only key's weight p is not 1 to the last bit, as the maximum that is
+    # taken off its score is rounded; so with u = 2^-24
+    # out = (p v) (1 / p): three roundings;
+    # dq = p (dp - (p dp) / p) k: two on dp = do v, and those of a product by
+    # what they leave; dk likewise by q;
+    # dv = p do, p from the logarithm, u (|s| + 5) off 1: the logarithm's
+    # rounding u |s|, u each for the sum's, its logarithm's and the
+    # difference's, and 2 u for the exponential.
+    u = 2.0 ** -24
+    with torch.no_grad():
+        assert ((out - v).abs() <= 4 * u * v.abs()).all()
+        assert (dq.abs() <= 4 * u * (do * v * k).abs()).all()
+        assert (dk.abs() <= 4 * u * (do * v * q).abs()).all()
+        assert ((dv - do).abs() <= 8 * u * (1 + (q * k).abs())
+                * do.abs()).all()
+    more = torch.zeros(most + 1, 1, 1, 1, device=DEV)
+    with pytest.raises(ValueError, match="one launch"):
+        ops.cross_attention(more, more, more)
+    # deep heads, whose gradients take twice the threads
+    deep = torch.zeros(2 ** 23, 1, 65, 1, device=DEV, dtype=BF16)
+    out = ops.cross_attention(deep.requires_grad_(), deep, deep)
+    with pytest.raises(ValueError, match="one launch"):
+        torch.autograd.grad(out.sum(), deep)
