@@ -64,9 +64,6 @@ struct Mma<__bf16> {
   static constexpr int kDepth = 16;     // channels of one first product
   using Op = bf16x8;
   __device__ static int seq(int i, int h) { return 16 * (i / 8) + 8 * h + i % 8; }
-  // channel of element j of the kk-th operand
-  __device__ static int channel(int kk, int j, int h) { return 16 * kk + 8 * h + j; }
-  __device__ static void put(Op& op, int j, float v) { op[j] = (__bf16)v; }
   __device__ static float get(const Op& op, int j) { return (float)op[j]; }
 
   // channels 16*kk.. of positions col..col+31, positions along the rows. The
@@ -117,8 +114,6 @@ struct Mma<float> {
   static constexpr int kDepth = 2;
   using Op = float;
   __device__ static int seq(int i, int h) { return 8 * (i / 4) + 4 * h + i % 4; }
-  __device__ static int channel(int kk, int j, int h) { return 2 * kk + h; }
-  __device__ static void put(Op& op, int, float v) { op = v; }
   __device__ static float get(const Op& op, int) { return op; }
   template <int STRIDE, bool SWAP = true>
   __device__ static Op first(const float* tile, int kk, int col) {
