@@ -9,6 +9,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 import _sequence_ref as ref
+import _sequence_walk as walk
 from seist_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -287,3 +288,113 @@ def test_attention_of_the_most_records():
     out = ops.cross_attention(deep.requires_grad_(), deep, deep)
     with pytest.raises(ValueError, match="one launch"):
         torch.autograd.grad(out.sum(), deep)
+
+
+# ---------------------------------------------------------------------------
+# variants by size, each against the formula
+# ---------------------------------------------------------------------------
+
+
+def _check_attention(shape, buckets, dtype, lens=None, table_grad=True,
+                     **more):
+    n, h, hkv, e, lq, lk = shape
+    q, k, v, do = _inputs((n, h, e, lq), (n, hkv, e, lk), (n, hkv, e, lk),
+                          (n, h, e, lq), dtype=dtype)
+    table = _inputs((h, buckets), dtype=dtype)[0] if buckets else None
+    if lens is not None:
+        lens = torch.tensor(lens, device=DEV, dtype=torch.int32)
+    want, bound = ref.attention(q, k, v, lens, table, dout=do, **more)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    if buckets and table_grad:
+        leaves.append(table.requires_grad_())
+    out = ops.cross_attention(q, k, v, lens, table, **more)
+    grads = torch.autograd.grad(out, leaves, do)
+    for name, got in zip(("out", "dq", "dk", "dv", "dtable"), (out,) + grads):
+        ref.assert_within(got, want[name], bound[name], name)
+
+
+@pytest.mark.parametrize("shape", [
+    (8, 16, 16, 64, 1050, 200), (8, 16, 16, 48, 1100, 333),
+    (8, 16, 16, 16, 1050, 300), (8, 32, 16, 24, 600, 515),
+])
+@pytest.mark.parametrize("lens", [None, [0, 1, 63, 129, 64, 197, 77, 200]])
+def test_attention_two_column_blocks(shape, lens):
+    """Queries enough for two blocks of columns a wave, and several staged
+    tiles of keys."""
+    _check_attention(shape, 0, BF16, lens)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("shape", [
+    (1, 2, 2, 16, 70, 50), (1, 4, 2, 32, 70, 700), (1, 2, 1, 24, 130, 20),
+    (2, 2, 2, 40, 33, 300), (1, 1, 1, 128, 100, 600),
+])
+def test_attention_with_a_bias_that_has_no_gradient(dtype, shape):
+    lens = [shape[5] - 9, shape[5]][:shape[0]]
+    _check_attention(shape, 8, dtype, lens, table_grad=False, max_distance=30)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("shape", [(70, 2, 1, 8, 1000, 20),
+                                   (600, 1, 1, 16, 40, 33),
+                                   (5, 3, 3, 8, 14001, 7)])
+def test_attention_table_of_many_rows(dtype, shape):
+    """A bias gradient of more than 512 row tiles, which two steps add up."""
+    _check_attention(shape, 8, dtype, max_distance=12)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("buckets", [0, 16])
+@pytest.mark.parametrize("shape", [(2, 8, 2, 128, 1, 300),
+                                   (1, 4, 4, 100, 7, 1100),
+                                   (3, 32, 1, 128, 1, 77)])
+def test_attention_few_rows_of_deep_heads(dtype, buckets, shape):
+    lens = [shape[5], 0, 31][:shape[0]]
+    more = dict(max_distance=40, query_start=50) if buckets else {}
+    _check_attention(shape, buckets, dtype, lens, **more)
+
+
+def _check_scan(dtype, n, c, length, memory, lens, reverse):
+    """Gates that keep a state for about ``memory`` samples, over a drift, so
+    that what comes from far shows."""
+    x, gate, dh = _inputs(*3 * [(n, c, length)])
+    state, ds = _inputs((n, c), (n, c), seed=1)
+    drift = torch.arange(length, device=DEV) / (3.0 * memory)
+    x = (x + drift.sin()).to(dtype)
+    dh = (dh + drift.cos()).to(dtype)
+    gate = (gate * 0.5 + math.log(memory)).to(dtype)
+    if lens is not None:
+        lens = torch.tensor(lens, device=DEV)
+    leaves = [t.requires_grad_() for t in (x, gate, state)]
+    out = ops.gated_scan(*leaves, lens, reverse)
+    grads = torch.autograd.grad(out, leaves, [dh, ds])
+    with torch.no_grad():
+        plain = ops.gated_scan(x, gate, state, lens, reverse)
+    want, bound = walk.scan(x, gate, state, lens, reverse, dh, ds)
+    names = ("h", "state", "dx", "dgate", "dstate")
+    for name, got in zip(names, plain):
+        ref.assert_within(got, want[name], bound[name], name + ", no gradient")
+    for name, got in zip(names, out + grads):
+        ref.assert_within(got, want[name], bound[name], name)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype,n,c,length,memory", [
+    (BF16, 1, 3, 7000, 2000),       # 4 waves a row, 2 segments
+    (FP32, 1, 3, 4000, 1000),
+    (BF16, 3, 2, 73733, 8000),      # 16 waves a row, 5 segments
+    (FP32, 3, 2, 40001, 4000),
+    (BF16, 1, 1, 1080001, 8000),    # 66 segments, over a wave's lanes
+    (FP32, 2, 1, 540001, 8000),
+    (BF16, 70, 64, 1000, 300),      # many rows, a wave each, two chunks
+    (FP32, 70, 64, 500, 200),
+    (BF16, 40, 30, 6000, 1000),     # 4 waves a row, the last chunk short
+    (FP32, 40, 30, 2900, 1000),
+])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_scan_variants(dtype, n, c, length, memory, reverse, ragged):
+    lens = None
+    if ragged:
+        lens = [(length * (2 * i + 1) // (2 * n) + 12345 * i) % (length + 1)
+                for i in range(n)]
+    _check_scan(dtype, n, c, length, memory, lens, reverse)

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import _sequence_ref as ref
+import _sequence_walk as walk
 from seist_amd import ops
 
 
@@ -103,3 +104,18 @@ def test_attention_pairs_out_whatever_their_scores(what):
     grads = torch.autograd.grad(out, leaves, do)
     for name, got in zip(("out", "dk", "dv", "dtable"), (out,) + grads[1:]):
         ref.assert_within(got, want[name], 2 * bound[name], name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lens", [None, [0, 31, 17]])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_walked_recurrence_is_the_formula(dtype, lens, reverse):
+    """What long records are compared with, against the steps one by one."""
+    x, gate, dh, state, ds = _inputs(*3 * [(3, 2, 31)], *2 * [(3, 2)])
+    args = [t.to(dtype) for t in (x, gate)] + [state, lens, reverse,
+                                               dh.to(dtype), ds]
+    for got, want in zip(walk.scan(*args), ref.scan(*args)):
+        assert got.keys() == want.keys()
+        for name in want:
+            torch.testing.assert_close(got[name], want[name], rtol=1e-12,
+                                       atol=1e-300)
