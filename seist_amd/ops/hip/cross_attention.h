@@ -345,8 +345,8 @@ __device__ __forceinline__ float bias_of(const Bias& b, int head, int d) {
 // whatever their scores are, and a NaN or an infinity plus -inf need not be
 // -inf; so such a wave looks the bias up once more for each score. For the
 // others that is a branch: pooled keys go from 28.5 to 29.7 us, training with
-// a bias from 273 to 275, and with a comparison and a selection for every
-// score to 31.2 and 284.
+// a bias stays at 273, and with a comparison and a selection for every score
+// they take 31.2 and 284.
 template <typename T>
 __device__ __forceinline__ float entry_of_lane(const Bias& b, int head) {
   const int lane = threadIdx.x & 63;

@@ -425,9 +425,19 @@ __device__ __forceinline__ void log_weights(const Args& p,
   const float scale = p.scale * kLog2e;
   const int far = p.bias.max_distance, step = p.bias.key_step;
   int side = 2;
-  if (LINED)
+  float add = 0.0f;
+  if (LINED) {
     side = beyond(p.bias, key0 * step - (from + 32 * SUBS - 1),
                   (key0 + 31) * step - from);
+    add = side > 0 ? behind : before;
+    if (side != 0 && add == -INFINITY) {  // all pairs are out
+#pragma unroll
+      for (int b = 0; b < SUBS; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) c[b][j] = -INFINITY;
+      return;
+    }
+  }
 #pragma unroll
   for (int b = 0; b < SUBS; ++b) {
     if (LINED && side == 0) {
@@ -444,20 +454,7 @@ __device__ __forceinline__ void log_weights(const Args& p,
                     l[j & 3];
         }
       }
-      if (holes) {
-        const int d1 = anew(d0);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int d = d1 - M::seq(j, 0);
-          // a query that is not there is zeros, and NaN by such a key
-          if (32 * b + M::seq(j, h) >= rows ||
-              line[line_at<true>(max(-far, min(d, far)))] == -INFINITY)
-            c[b][j] = -INFINITY;
-        }
-      }
     } else {
-      const float add = !LINED ? 0.0f : side > 0 ? behind : before;
-      if (LINED && add == -INFINITY) c[b] = f32x16{};
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 l = *(const f32x4*)(lses + 32 * b + M::seq(4 * g, h));
@@ -465,6 +462,21 @@ __device__ __forceinline__ void log_weights(const Args& p,
         for (int j = 4 * g; j < 4 * g + 4; ++j)
           c[b][j] =
               fmaf(c[b][j], scale, LINED ? add - l[j & 3] : -l[j & 3]);
+      }
+    }
+  }
+  if (LINED && side == 0 && holes) {
+#pragma unroll
+    for (int b = 0; b < SUBS; ++b) {
+      const int d0 = anew((key0 + (lane & 31)) * step - from - 32 * b -
+                          M::seq(0, h));
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int d = d0 - M::seq(j, 0);
+        // a query that is not there is zeros, and NaN by such a key
+        if (32 * b + M::seq(j, h) >= rows ||
+            line[line_at<true>(max(-far, min(d, far)))] == -INFINITY)
+          c[b][j] = -INFINITY;
       }
     }
   }
