@@ -122,11 +122,15 @@ __device__ __forceinline__ void add_diagonals(const Bias& b,
 // In heads of few channels that rounding shows whatever the keys' number: k's
 // mean under p is q / E. So for up to 32 channels in bf16 the sums over keys
 // of ds and of p k are kept as well: the first would be zero, and times the
-// second it is what dq is off by; added to delta, it sets that right. Up to
-// 16 channels the sum that dq is mended by is of the rounded ds, so that their
-// roundings do not meet k's mean either. Error of dq against 64 bits, 4347 by
-// 1024, heads of 24: 0.00247 and 0.00242, and a training step takes 264 and
-// not 249 us (291 with a DELTA launch, which a cut over keys needs).
+// second it is what dq is off by; added to delta, it sets that right. Errors
+// of dq against 64 bits, in those that rounding the exact dq leaves: 17 to 32
+// channels 1.45 to 1.48 and 1.47 to 1.55 without, for 228 and 205 us of a
+// backward pass of 32 x 8 heads, 1024 by 1024 (and a DELTA launch where keys
+// are cut).
+// Up to 16 channels the roundings of ds meet k's mean as well, and what they
+// add up to is taken off with it, whoever found delta: 1.40, the sqrt(2) of
+// two independent roundings, where it was 1.48 at 16 channels, 1.6 at 8 and
+// 1.65 at 4. TABLE takes 173 and not 144 us (16 x 8 heads of 16, 2048 by 1000).
 //
 // Bound as the forward kernel is: 4096 x 4096, 64 heads of 128 on 16, 820 us,
 // 1006 TFLOP/s; (8, 8, 2048 x 1000 at most) heads of 64 with a bias 43 us for
@@ -181,6 +185,7 @@ void attend_dq_kernel(Args p) {
   constexpr bool MEND = FIND == DQ && sizeof(T) == 2 && ED <= 32;
   const bool given = FIND == TABLE || (MEND && p.deltas != nullptr);
   const bool mend = MEND && !given;
+  constexpr bool EVEN = FIND != DELTA && sizeof(T) == 2 && ED == 16;
   const bool few = FIND == DQ && !MEND && total <= 32;
   if (given && live) {
     for (int s = 0; s < p.splits; ++s) {
@@ -189,6 +194,7 @@ void attend_dq_kernel(Args p) {
       weight += of[rows];
     }
     if (weight != 0.0f) delta /= weight;
+    weight = 0.0f;
   }
   if (FIND == DQ && !given && !few) {
     typename M::Op o[ED / M::kDepth];
@@ -226,7 +232,7 @@ void attend_dq_kernel(Args p) {
   const bool holes = LINED && takes_out(entry);
   f32x16 acc[DB] = {};
   f32x16 mean = {};    // sum of p k
-  float excess = 0.0f, rounded = 0.0f;  // sums of ds
+  float excess = 0.0f;  // sum of ds
   const float scale = p.scale * kLog2e;
   const T* kb = (const T*)p.k + n * p.kn + hk * p.kh;
   const T* vb = (const T*)p.v + n * p.vn + hk * p.vh;
@@ -253,6 +259,18 @@ void attend_dq_kernel(Args p) {
       vs.load(vb, at + POS, end, tid);
     }
     if (i0 >= p.Lq) continue;  // no query of this wave's
+    // Up to 16 channels are half of a product's rows. Ones in the others make
+    // the weights' sum of what they weigh, over both halves' keys, in all of
+    // rows 16.. (element 8 and its like).
+    auto keys_and_ones = [&](int col) {
+      auto left = M::template second<Staged::kStride, ED>(kt, 0, col);
+      if constexpr (EVEN) {
+        if (lane & 16)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) left.a[0][j] = left.a[1][j] = (__bf16)1.0f;
+      }
+      return left;
+    };
 #pragma unroll 1
     for (int col = 0; col < POS && at + col < end; col += 32) {
       const int key0 = at + col;
@@ -305,13 +323,14 @@ void attend_dq_kernel(Args p) {
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j) ds[j] = __builtin_amdgcn_exp2f(ds[j]);
-      if (mend) {
+      if (mend || EVEN) {
         typename M::Right pr;
         M::right(pr, ds);
-        mean = M::mul(M::template second<Staged::kStride, ED>(kt, 0, col), pr,
-                      mean);
+        mean = M::mul(keys_and_ones(col), pr, mean);
+        if (!EVEN) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) weight += ds[j];
+          for (int j = 0; j < 16; ++j) weight += ds[j];
+        }
       }
       if (FIND == DELTA) {
 #pragma unroll
@@ -346,32 +365,28 @@ void attend_dq_kernel(Args p) {
         if (side > 0) ds_behind += all;
         else ds_before += all;
       }
-      if (mend) {
+      if (mend || EVEN) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) excess += ds[j];
       }
       typename M::Right pr;
       M::right(pr, ds);
-      if constexpr (MEND && ED == 16) {
-        if (mend) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) rounded += (float)pr[j / 8][j % 8];
-        }
-      }
 #pragma unroll
       for (int d = 0; d < DB; ++d)
         acc[d] = M::mul(
-            M::template second<Staged::kStride, ED>(kt, 32 * d, col), pr,
-            acc[d]);
+            EVEN ? keys_and_ones(col)
+                 : M::template second<Staged::kStride, ED>(kt, 32 * d, col),
+            pr, acc[d]);
     }
   }
-  if (mend) {
-    weight = both_sum(weight);
+  if (mend || EVEN) {
     excess = both_sum(excess);
-    rounded = ED == 16 ? both_sum(rounded) : excess;
+    weight = EVEN ? mean[8] : both_sum(weight);
     const float by = weight != 0.0f ? 1.0f / weight : 0.0f;
-    delta += excess * by;
-    acc[0] -= mean * (rounded * by);
+    float off = excess;
+    if (EVEN) off = mend ? acc[0][8] : acc[0][8] - excess;
+    if (mend) delta += excess * by;
+    acc[0] -= mean * (off * by);
   }
   if (FIND == DELTA) {
     delta = both_sum(delta);

@@ -398,3 +398,27 @@ def test_scan_variants(dtype, n, c, length, memory, reverse, ragged):
         lens = [(length * (2 * i + 1) // (2 * n) + 12345 * i) % (length + 1)
                 for i in range(n)]
     _check_scan(dtype, n, c, length, memory, lens, reverse)
+
+
+@pytest.mark.parametrize("e", [8, 11, 16])
+@pytest.mark.parametrize("h,hkv,lq,lk,buckets", [
+    (4, 4, 333, 700, 0),            # keys cut, so a delta walked beforehand
+    (4, 2, 777, 1024, 0),
+    (4, 4, 333, 700, 16),           # the bias has a gradient
+    (64, 64, 1100, 300, 16),        # the same, uncut
+    (64, 64, 1100, 300, 0),
+])
+def test_attention_gradients_of_small_heads(e, h, hkv, lq, lk, buckets):
+    """dq in bf16 has two independent roundings of one size, ds's and its own:
+    sqrt(2) of the result's alone. What all of a query's ds are off by together
+    would meet the mean of the keys, which small heads do not average out; 1.5
+    leaves it a twentieth of the variance, and the sums' scatter room."""
+    q, k, v, do = _inputs((1, h, e, lq), (1, hkv, e, lk), (1, hkv, e, lk),
+                          (1, h, e, lq), dtype=BF16)
+    table = _inputs((h, buckets), dtype=BF16)[0] if buckets else None
+    want, _ = ref.attention(q, k, v, None, table, max_distance=64, dout=do)
+    leaves = [t.requires_grad_() for t in (q, k, v, table) if t is not None]
+    out = ops.cross_attention(q, k, v, None, table, max_distance=64)
+    dq = torch.autograd.grad(out, leaves, do)[0]
+    least = (want["dq"].to(BF16).double() - want["dq"]).norm()
+    assert (dq.double() - want["dq"]).norm() <= 1.5 * least
