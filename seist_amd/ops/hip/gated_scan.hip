@@ -86,16 +86,24 @@ __device__ __forceinline__ void gates(float g, float& a, float& keep) {
 
 // a lane's samples of scan index s0.., in the words that they fill in
 // memory, so that a load is not waited for before its samples are used; rows
-// start anywhere, so the 16-byte accesses are not aligned
+// start anywhere, so the 16-byte accesses are not aligned. Rows of 16 bytes at
+// most (SHORT), a lane each, go by samples. In others a lane that passes the
+// row's end reads the last 16 bytes before it, which settle() moves to their
+// places when they are used, and the one lane that the end falls into writes
+// by samples. 52 million samples in bf16 in rows of 8192, 6000, 1500, 300 and
+// 100 take 67, 69, 93, 122 and 102 us (98, 99, 142, 184 and 141 backward);
+// with a row's last chunk by samples, 67, 84, 170, 166 and 174 (97, 139, 285,
+// 282 and 285).
 template <typename T>
 struct Items {
   static constexpr int kEach = 4 / sizeof(T);  // samples of a word
   unsigned w[kItems<T> / kEach];
-  template <bool REV>
-  __device__ __forceinline__ void load(const T* row, int s0, int L,
-                                       bool whole) {
-    if (whole) {
-      __builtin_memcpy(w, row + (REV ? L - kItems<T> - s0 : s0), sizeof(w));
+  template <bool REV, bool SHORT>
+  __device__ __forceinline__ void load(const T* row, int s0, int L) {
+    if (!SHORT || L == kItems<T>) {
+      __builtin_memcpy(
+          w, row + (REV ? max(L - kItems<T> - s0, 0) : min(s0, L - kItems<T>)),
+          sizeof(w));
     } else {
 #pragma unroll
       for (int k = 0; k < kItems<T>; ++k) {  // as they come in memory
@@ -105,6 +113,25 @@ struct Items {
         if (k % kEach == 0) w[k / kEach] = v;
         else w[k / kEach] |= v << 16;
       }
+    }
+  }
+  // in steps of 2 words, 1 word, half a word; what has no sample is any
+  template <bool REV>
+  __device__ __forceinline__ void settle(int s0, int L) {
+    const int over = max(s0 + kItems<T> - L, 0);
+    const bool two = over & (2 * kEach), one = over & kEach;
+    const bool half = kEach == 2 && (over & 1);
+    auto word = [&](int k) -> unsigned& { return w[REV ? 3 - k : k]; };
+#pragma unroll
+    for (int k = 0; k < 2; ++k) word(k) = two ? word(k + 2) : word(k);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) word(k) = one ? word(k + 1) : word(k);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const unsigned next = k < 3 ? word(k + 1) : 0;
+      const unsigned moved =
+          REV ? word(k) << 16 | next >> 16 : word(k) >> 16 | next << 16;
+      word(k) = half ? moved : word(k);
     }
   }
   template <bool REV>
@@ -124,7 +151,7 @@ struct Items {
   template <bool REV>
   __device__ __forceinline__ void store(T* row, int s0, int L,
                                         bool whole) const {
-    if (whole) {
+    if (whole || s0 + kItems<T> <= L) {
       __builtin_memcpy(row + (REV ? L - kItems<T> - s0 : s0), w, sizeof(w));
     } else {
 #pragma unroll
@@ -247,6 +274,7 @@ __device__ __forceinline__ float through(const float* maps, int segments,
 template <typename T, int LPR, int W, bool REV>
 struct Place {
   static constexpr int kChunk = LPR * W * kItems<T>;
+  static constexpr bool kShort = LPR == 1;
   const ScanArgs& p;
   long row, n, c;
   int lane, seg, first, last, begin, end, len;
@@ -315,11 +343,15 @@ struct Place {
 // sample passes the state on
 template <bool REV, bool FULL, typename T, typename P>
 __device__ __forceinline__ void take(const P& at, int chunk,
-                                     const Items<T>& gate,
-                                     const Items<T>& more, bool given,
+                                     Items<T> gate, Items<T> more,
+                                     bool given,
                                      float (&a)[kItems<T>],
                                      float (&keep)[kItems<T>],
                                      float (&m)[kItems<T>]) {
+  if (!FULL && !P::kShort) {
+    gate.template settle<REV>(at.start(chunk), at.p.L);
+    more.template settle<REV>(at.start(chunk), at.p.L);
+  }
 #pragma unroll
   for (int i = 0; i < kItems<T>; ++i) {
     gates(gate.template at<REV>(i), a[i], keep[i]);
@@ -356,9 +388,9 @@ SCAN_KERNEL scan_map_kernel(ScanArgs p) {
   const T *x = at.x(), *gate = at.gate();
   Items<T> xi, gi;
   auto fetch = [&](int chunk) {
-    const bool whole = at.whole(chunk);
-    gi.template load<REV>(gate, at.start(chunk), p.L, whole);
-    xi.template load<REV>(x, at.start(chunk), p.L, whole);
+    const int s0 = at.start(chunk);
+    gi.template load<REV, at.kShort>(gate, s0, p.L);
+    xi.template load<REV, at.kShort>(x, s0, p.L);
   };
   if (at.begin < at.end) fetch(at.begin);
   Map m = {1.0f, 0.0f};
@@ -390,9 +422,9 @@ SCAN_KERNEL scan_map_back_kernel(ScanArgs p) {
   const T *dh = at.dh(), *gate = at.gate();
   Items<T> di, gi;
   auto fetch = [&](int chunk) {
-    const bool whole = at.whole(chunk);
-    gi.template load<REV>(gate, at.start(chunk), p.L, whole);
-    if (dh) di.template load<REV>(dh, at.start(chunk), p.L, whole);
+    const int s0 = at.start(chunk);
+    gi.template load<REV, at.kShort>(gate, s0, p.L);
+    if (dh) di.template load<REV, at.kShort>(dh, s0, p.L);
   };
   if (at.begin < at.end) fetch(at.end - 1);
   Map m = {1.0f, 0.0f};
@@ -424,9 +456,9 @@ SCAN_KERNEL scan_kernel(ScanArgs p) {
   T* out = (T*)p.out + at.row * p.L;
   Items<T> xi, gi;
   auto fetch = [&](int chunk) {
-    const bool whole = at.whole(chunk);
-    gi.template load<REV>(gate, at.start(chunk), p.L, whole);
-    xi.template load<REV>(x, at.start(chunk), p.L, whole);
+    const int s0 = at.start(chunk);
+    gi.template load<REV, at.kShort>(gate, s0, p.L);
+    xi.template load<REV, at.kShort>(x, s0, p.L);
   };
   if (at.begin < at.end) fetch(at.begin);
   float state = p.state ? p.state[at.row] : 0.0f;
@@ -478,10 +510,10 @@ SCAN_KERNEL scan_back_kernel(ScanArgs p) {
   Items<T> xi, gi, di;
   float mark = 0.0f;
   auto fetch = [&](int chunk) {
-    const bool whole = at.whole(chunk);
-    gi.template load<REV>(gate, at.start(chunk), p.L, whole);
-    xi.template load<REV>(x, at.start(chunk), p.L, whole);
-    if (dh) di.template load<REV>(dh, at.start(chunk), p.L, whole);
+    const int s0 = at.start(chunk);
+    gi.template load<REV, at.kShort>(gate, s0, p.L);
+    xi.template load<REV, at.kShort>(x, s0, p.L);
+    if (dh) di.template load<REV, at.kShort>(dh, s0, p.L);
     mark = marks[chunk];
   };
   if (at.begin < at.end) fetch(at.end - 1);
@@ -495,6 +527,8 @@ SCAN_KERNEL scan_back_kernel(ScanArgs p) {
       const float state = mark;
       float xs[kItems<T>], a[kItems<T>], keep[kItems<T>], d[kItems<T>];
       const Items<T> gn = gi, xn = xi;
+      if (!FULL && !at.kShort)
+        di.template settle<REV>(at.start(chunk), p.L);
 #pragma unroll
       for (int i = 0; i < kItems<T>; ++i)
         d[i] = dh ? di.template at<REV>(i) : 0.0f;

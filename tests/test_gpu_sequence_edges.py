@@ -422,3 +422,13 @@ def test_attention_gradients_of_small_heads(e, h, hkv, lq, lk, buckets):
     dq = torch.autograd.grad(out, leaves, do)[0]
     least = (want["dq"].to(BF16).double() - want["dq"]).norm()
     assert (dq.double() - want["dq"]).norm() <= 1.5 * least
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_scan_lengths_by_the_sample(dtype, reverse):
+    """A row's end at each place of a lane's samples, with one lane a row, 16,
+    64, 4 waves and several chunks; rows follow one another without a gap."""
+    for base in (1, 9, 17, 60, 120, 500, 1020, 2040, 4090, 6140):
+        for length in range(base, base + 9):
+            _check_scan(dtype, 3, 5, length, 40, None, reverse)
