@@ -10,6 +10,7 @@
 #include <climits>
 
 #include "sa_common.h"
+#include "sa_tensor.h"
 
 namespace attend {
 
@@ -508,9 +509,9 @@ struct Call {
 
 inline Args args_of(const Call& c) {
   Args p = {};
-  p.q = c.q.data_ptr();
-  p.k = c.k.data_ptr();
-  p.v = c.v.data_ptr();
+  p.q = sa::memory_of(c.q);
+  p.k = sa::memory_of(c.k);
+  p.v = sa::memory_of(c.v);
   p.qn = c.q.stride(0), p.qh = c.q.stride(1), p.qe = c.q.stride(2);
   p.kn = c.k.stride(0), p.kh = c.k.stride(1), p.ke = c.k.stride(2);
   p.vn = c.v.stride(0), p.vh = c.v.stride(1), p.ve = c.v.stride(2);
@@ -518,10 +519,10 @@ inline Args args_of(const Call& c) {
   p.G = p.H / p.Hkv;
   p.E = c.q.size(2), p.Lq = c.q.size(3), p.Lk = c.k.size(3);
   p.scale = (float)c.scale;
-  if (c.lengths.defined()) p.lengths = c.lengths.data_ptr<int>();
+  if (c.lengths.defined()) p.lengths = sa::memory_of<int>(c.lengths);
   if (c.table.defined()) {
     Bias& b = p.bias;
-    b.table = c.table.data_ptr();
+    b.table = sa::memory_of(c.table);
     b.buckets = c.table.size(1);
     b.exact = b.buckets / 4;
     b.max_distance = c.max_distance;

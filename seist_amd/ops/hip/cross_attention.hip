@@ -542,8 +542,8 @@ std::vector<at::Tensor> forward(const Call& c, bool stats) {
   if (stats) lse = at::empty({p.N, p.H, p.Lq}, f32);
   if (out.numel() == 0) return {out, lse};
   const auto stream = at::hip::getCurrentHIPStream().stream();
-  p.out = out.data_ptr();
-  p.lse = stats ? lse.data_ptr<float>() : nullptr;
+  p.out = sa::memory_of(out);
+  p.lse = stats ? sa::memory_of<float>(lse) : nullptr;
   const long pairs = (long)p.N * p.Hkv;
   const bool few = (long)p.G * p.Lq <= 32;
   // two blocks of columns a wave where that still leaves every compute unit
@@ -562,7 +562,7 @@ std::vector<at::Tensor> forward(const Call& c, bool stats) {
   if (p.splits > 1) {
     const long sums = p.splits * pairs * p.E * rows;
     part = at::empty({sums + p.splits * pairs * 2 * rows}, f32);
-    p.part = part.data_ptr<float>();
+    p.part = sa::memory_of<float>(part);
     p.stat = p.part + sums;
   }
   const long blocks = pairs * p.splits * p.tiles;
@@ -613,12 +613,6 @@ std::string shape_of(const at::Tensor& t) {
   return c10::str(t.sizes(), " ", t.scalar_type(), " on ", t.device());
 }
 
-// whether forward mode carries a derivative along with t: the kernels would
-// drop it
-bool has_tangent(const at::Tensor& t) {
-  return t.defined() && t._fw_grad(/*level=*/0).defined();
-}
-
 // What the kernels take for granted. Lengths outside 0..Lk are held to it by
 // the kernels.
 Call checked(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
@@ -640,9 +634,9 @@ Call checked(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
   TORCH_CHECK_VALUE(q.is_cuda() && k.device() == q.device() &&
                         v.device() == q.device(),
                     "cross_attention: q, k and v have to be on one device");
-  TORCH_CHECK(!has_tangent(q) && !has_tangent(k) &&
-                  !has_tangent(v) &&
-                  !(table.has_value() && has_tangent(*table)),
+  TORCH_CHECK(!sa::has_tangent(q) && !sa::has_tangent(k) &&
+                  !sa::has_tangent(v) &&
+                  !(table.has_value() && sa::has_tangent(*table)),
               "cross_attention: forward-mode derivatives are not available");
   const long H = q.size(1), Hkv = k.size(1), E = q.size(2), Lq = q.size(3),
              Lk = k.size(3);
@@ -736,7 +730,7 @@ class CrossAttention : public torch::autograd::Function<CrossAttention> {
       torch::autograd::variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "cross_attention: second derivatives are not available");
-    TORCH_CHECK(!has_tangent(grads[0]),
+    TORCH_CHECK(!sa::has_tangent(grads[0]),
                 "cross_attention: forward-mode derivatives are not available");
     const auto s = ctx->get_saved_variables();
     const auto where = ctx->saved_data["where"].toIntVector();

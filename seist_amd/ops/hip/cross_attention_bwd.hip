@@ -865,14 +865,14 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
   }
   const auto stream = at::hip::getCurrentHIPStream().stream();
   auto delta = at::empty({p.N, p.H, p.Lq}, f32);
-  p.o = out.data_ptr();
-  p.lse = lse.data_ptr<float>();
-  p.delta = delta.data_ptr<float>();
-  p.dout = dout.data_ptr();
+  p.o = sa::memory_of(out);
+  p.lse = sa::memory_of<float>(lse);
+  p.delta = sa::memory_of<float>(delta);
+  p.dout = sa::memory_of(dout);
   p.dn = dout.stride(0), p.dh = dout.stride(1), p.de = dout.stride(2);
   const long pairs = (long)p.N * p.Hkv;
 
-  p.out = dq.data_ptr();
+  p.out = sa::memory_of(dq);
   // with a bias, a workgroup's rows are one head's
   p.pad = round_up(p.Lq, p.bias.table ? 128 : 32);
   p.tiles = sa::ceil_div((long)p.G * p.pad, 128);
@@ -882,15 +882,15 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
   at::Tensor part, sums, deltas;
   if (p.splits > 1) {
     part = at::empty({p.splits, c.q.numel()}, f32);
-    p.part = part.data_ptr<float>();
+    p.part = sa::memory_of<float>(part);
   }
   if (walked) {
     deltas = at::empty({p.splits, 2, p.N, p.H, p.Lq}, f32);
-    p.deltas = deltas.data_ptr<float>();
+    p.deltas = sa::memory_of<float>(deltas);
   }
   if (table) {
     sums = at::empty({p.N * p.splits, p.H, p.pad / 128, p.bias.buckets}, f32);
-    p.dbias = sums.data_ptr<float>();
+    p.dbias = sa::memory_of<float>(sums);
   }
   const size_t line = (2 * p.bias.max_distance + 1) * 4;
   with_type(c.q.scalar_type(), [&](auto zero) {
@@ -921,7 +921,7 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
     });
     if (p.splits > 1) {
       sum_splits_kernel<T><<<sa::ceil_div(c.q.numel(), 256), 256, 0, stream>>>(
-          p.part, (T*)dq.data_ptr(), c.q.numel(), p.splits);
+          p.part, sa::memory_of<T>(dq), c.q.numel(), p.splits);
       SA_CHECK_HIP(hipGetLastError());
     }
     if (table) {
@@ -931,14 +931,14 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
       const dim3 grid(p.H, pieces);
       if (pieces == 1) {
         sum_table_kernel<T><<<grid, 256, 0, stream>>>(
-            p.dbias, (T*)dt.data_ptr(), of, p.H, tiles, p.bias.buckets);
+            p.dbias, sa::memory_of<T>(dt), of, p.H, tiles, p.bias.buckets);
       } else {
         auto some = at::empty({p.H, pieces, p.bias.buckets}, f32);
         sum_table_kernel<float><<<grid, 256, 0, stream>>>(
-            p.dbias, some.data_ptr<float>(), of, p.H, tiles,
+            p.dbias, sa::memory_of<float>(some), of, p.H, tiles,
             p.bias.buckets);
         sum_table_kernel<T><<<dim3(p.H, 1), 256, 0, stream>>>(
-            some.data_ptr<float>(), (T*)dt.data_ptr(), 1, p.H, pieces,
+            sa::memory_of<float>(some), sa::memory_of<T>(dt), 1, p.H, pieces,
             p.bias.buckets);
       }
       SA_CHECK_HIP(hipGetLastError());
@@ -946,8 +946,8 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
   });
   if (!kv) return {dq, dk, dv, dt};
 
-  p.dk = dk.data_ptr();
-  p.dv = dv.data_ptr();
+  p.dk = sa::memory_of(dk);
+  p.dv = sa::memory_of(dv);
   p.tiles = sa::ceil_div(p.Lk, 128);
   with_type(c.q.scalar_type(), [&](auto zero) {
     using T = decltype(zero);
@@ -958,7 +958,7 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
       p.splits = cut(pairs * p.tiles, (long)p.G * p.pad, POS, &p.per_split);
       if (p.splits > 1) {
         part = at::empty({2, p.splits, c.k.numel()}, f32);
-        p.part = part.data_ptr<float>();
+        p.part = sa::memory_of<float>(part);
       }
       const long blocks = pairs * p.splits * p.tiles;
       const size_t lines =
@@ -984,9 +984,9 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& out,
     if (p.splits > 1) {
       const int grid = sa::ceil_div(c.k.numel(), 256);
       sum_splits_kernel<T><<<grid, 256, 0, stream>>>(
-          p.part, (T*)dk.data_ptr(), c.k.numel(), p.splits);
+          p.part, sa::memory_of<T>(dk), c.k.numel(), p.splits);
       sum_splits_kernel<T><<<grid, 256, 0, stream>>>(
-          p.part + p.splits * c.k.numel(), (T*)dv.data_ptr(), c.k.numel(),
+          p.part + p.splits * c.k.numel(), sa::memory_of<T>(dv), c.k.numel(),
           p.splits);
       SA_CHECK_HIP(hipGetLastError());
     }

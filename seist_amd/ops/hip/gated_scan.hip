@@ -34,6 +34,7 @@
 #include <c10/core/DeviceGuard.h>
 
 #include "sa_common.h"
+#include "sa_tensor.h"
 
 namespace gated_scan {
 namespace {
@@ -664,9 +665,9 @@ struct Call {
 
 ScanArgs args_of(const Call& c, const Deal& deal) {
   ScanArgs p = {};
-  p.x = c.x.data_ptr();
-  p.gate = c.gate.data_ptr();
-  if (c.lengths.defined()) p.lengths = c.lengths.data_ptr<int>();
+  p.x = sa::memory_of(c.x);
+  p.gate = sa::memory_of(c.gate);
+  if (c.lengths.defined()) p.lengths = sa::memory_of<int>(c.lengths);
   p.xn = c.x.stride(0);
   p.xc = c.x.stride(1);
   p.gn = c.gate.stride(0);
@@ -693,16 +694,16 @@ std::vector<at::Tensor> forward(const Call& c, bool marked) {
   ScanArgs p = args_of(c, deal);
   if (marked) {
     marks = at::empty({rows, deal.chunks}, f32);
-    p.marks = marks.data_ptr<float>();
+    p.marks = sa::memory_of<float>(marks);
   }
-  if (c.state.defined()) p.state = c.state.data_ptr<float>();
-  p.out = h.data_ptr();
-  p.last = last.data_ptr<float>();
+  if (c.state.defined()) p.state = sa::memory_of<float>(c.state);
+  p.out = sa::memory_of(h);
+  p.last = sa::memory_of<float>(last);
   const auto stream = at::hip::getCurrentHIPStream().stream();
   const auto type = c.x.scalar_type();
   if (deal.segments > 1) {
     maps = at::empty({rows, deal.segments, 2}, f32);
-    p.maps = p.maps_out = maps.data_ptr<float>();
+    p.maps = p.maps_out = sa::memory_of<float>(maps);
     launch(MAP, type, c.reverse, p, deal, stream);
   }
   launch(SCAN, type, c.reverse, p, deal, stream);
@@ -722,18 +723,18 @@ std::vector<at::Tensor> backward(const Call& c, const at::Tensor& marks,
   if (rows == 0) return {dx, dgate, first};
   const Deal deal(rows, c.x.size(2), 16 / c.x.element_size());
   ScanArgs p = args_of(c, deal);
-  if (dh.defined()) p.dh = dh.data_ptr();
-  if (dstate.defined()) p.dstate = dstate.data_ptr<float>();
-  p.marks = marks.data_ptr<float>();
-  p.out = dx.data_ptr();
-  p.out2 = dgate.data_ptr();
-  p.last = first.data_ptr<float>();
+  if (dh.defined()) p.dh = sa::memory_of(dh);
+  if (dstate.defined()) p.dstate = sa::memory_of<float>(dstate);
+  p.marks = sa::memory_of<float>(marks);
+  p.out = sa::memory_of(dx);
+  p.out2 = sa::memory_of(dgate);
+  p.last = sa::memory_of<float>(first);
   const auto stream = at::hip::getCurrentHIPStream().stream();
   const auto type = c.x.scalar_type();
   at::Tensor maps;
   if (deal.segments > 1) {
     maps = at::empty({rows, deal.segments, 2}, f32);
-    p.maps = p.maps_out = maps.data_ptr<float>();
+    p.maps = p.maps_out = sa::memory_of<float>(maps);
     launch(MAP_BACK, type, c.reverse, p, deal, stream);
   }
   launch(SCAN_BACK, type, c.reverse, p, deal, stream);
@@ -746,12 +747,6 @@ std::string shape_of(const at::Tensor& t) {
 
 at::Tensor along_samples(const at::Tensor& t) {
   return t.stride(2) == 1 ? t : t.contiguous();
-}
-
-// whether forward mode carries a derivative along with t: the kernels would
-// drop it
-bool has_tangent(const at::Tensor& t) {
-  return t.defined() && t._fw_grad(/*level=*/0).defined();
 }
 
 // What the kernels take for granted. Lengths outside 0..L are held to it by
@@ -771,8 +766,8 @@ Call checked(const at::Tensor& x, const at::Tensor& gate,
       type, " and ", gate.scalar_type());
   TORCH_CHECK_VALUE(x.is_cuda() && gate.device() == x.device(),
                     "gated_scan: x and gate have to be on one device");
-  TORCH_CHECK(!has_tangent(x) && !has_tangent(gate) &&
-                  !(state.has_value() && has_tangent(*state)),
+  TORCH_CHECK(!sa::has_tangent(x) && !sa::has_tangent(gate) &&
+                  !(state.has_value() && sa::has_tangent(*state)),
               "gated_scan: forward-mode derivatives are not available");
   TORCH_CHECK_VALUE(x.size(2) < (1L << 30) &&
                         x.size(0) * x.size(1) < (1L << 24),
@@ -823,7 +818,7 @@ class GatedScan : public torch::autograd::Function<GatedScan> {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "gated_scan: second derivatives are not available");
     for (const auto& g : grads)
-      TORCH_CHECK(!has_tangent(g),
+      TORCH_CHECK(!sa::has_tangent(g),
                   "gated_scan: forward-mode derivatives are not available");
     const auto s = ctx->get_saved_variables();
     const Call call = {s[0], s[1], {}, s[2],

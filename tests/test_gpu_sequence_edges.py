@@ -7,6 +7,8 @@ import warnings
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
+from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import _sequence_ref as ref
 import _sequence_walk as walk
@@ -129,6 +131,34 @@ def test_scan_traced(dtype, grad):
         grads = torch.autograd.grad(outs, leaves, [dh, ds])
         for name, got in zip(("dx", "dgate", "dstate"), grads):
             ref.assert_within(got, want[name], bound[name], name)
+
+
+def test_calls_that_are_recorded_or_fake():
+    """Recorded by the dispatcher, the plain steps are; under a mode that
+    puts fake tensors in the place of results, and on fake tensors, no kernel
+    runs, which would write to their null pointers."""
+    q, k, x = _inputs((1, 2, 4, 5), (1, 2, 4, 6), (1, 2, 9))
+    want, bound = ref.attention(q + 1, k + 1, k + 1)
+    made = make_fx(lambda q, k: ops.cross_attention(q, k, k))(q, k)
+    ref.assert_within(made(q + 1, k + 1), want["out"], bound["out"], "out")
+    want, bound = ref.scan(x + 1, x + 1)
+    made = make_fx(lambda x: ops.gated_scan(x, x)[0])(x)
+    ref.assert_within(made(x + 1), want["h"], bound["h"], "h")
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        for args in ((q, k), (mode.from_tensor(q), mode.from_tensor(k))):
+            out = ops.cross_attention(args[0], args[1], args[1])
+            assert isinstance(out, FakeTensor) and out.shape == q.shape
+        h, last = ops.gated_scan(x, x)
+        assert isinstance(h, FakeTensor) and last.shape == (1, 2)
+    for f, t in ((lambda q: ops.cross_attention(q, k, k), q),
+                 (lambda x: ops.gated_scan(x, x)[0], x)):
+        with pytest.raises(RuntimeError, match="no memory"):
+            torch.func.functionalize(f)(t)
+        y = f(t.clone().requires_grad_())
+        with FakeTensorMode(allow_non_fake_inputs=True), \
+                pytest.raises(RuntimeError, match="no memory"):
+            y.sum().backward()
+    torch.cuda.synchronize()
 
 
 # ---------------------------------------------------------------------------

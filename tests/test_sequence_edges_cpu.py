@@ -6,6 +6,8 @@ import warnings
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import _sequence_ref as ref
 import _sequence_walk as walk
@@ -119,3 +121,42 @@ def test_walked_recurrence_is_the_formula(dtype, lens, reverse):
         for name in want:
             torch.testing.assert_close(got[name], want[name], rtol=1e-12,
                                        atol=1e-300)
+
+
+def test_tensors_without_memory_are_not_given_to_kernels():
+    """Fake tensors that say they are on a GPU: shapes and types come back and
+    no kernel runs, in their mode and outside of it."""
+    with FakeTensorMode():
+        q, k = (torch.empty(2, 4, 8, n, device="cuda", dtype=torch.bfloat16)
+                for n in (5, 7))
+        x = torch.empty(2, 3, 9, device="cuda")
+        lens = torch.empty(2, device="cuda", dtype=torch.int32)
+        table = torch.empty(4, 8, device="cuda", dtype=torch.bfloat16)
+        outs = [(ops.cross_attention(q, k, k, lens, table),)
+                + ops.gated_scan(x, x, None, lens)]
+    outs.append((ops.cross_attention(q, k, k),) + ops.gated_scan(x, x))
+    for out, h, last in outs:
+        assert out.shape == q.shape and out.dtype == torch.bfloat16
+        assert h.shape == x.shape and last.shape == (2, 3)
+        assert all(t.device.type == "cuda" for t in (out, h, last))
+
+
+def test_recorded_calls_compute_their_own_inputs():
+    q, k, x = _inputs((1, 2, 4, 5), (1, 2, 4, 6), (1, 2, 9))
+    for mode in ("real", "fake"):
+        for f, args in ((lambda q, k: ops.cross_attention(q, k, k), (q, k)),
+                        (lambda x: ops.gated_scan(x, x)[0], (x,))):
+            made = make_fx(f, tracing_mode=mode)(*args)
+            args = [t + 1 for t in args]
+            assert torch.equal(made(*args), f(*args))
+
+
+@pytest.mark.skipif(not ops.has_ext(), reason="the extension is not built")
+def test_the_extension_refuses_tensors_without_memory():
+    with FakeTensorMode():
+        q = torch.empty(1, 2, 4, 5, device="cuda")
+        x = torch.empty(1, 2, 5, device="cuda")
+        with pytest.raises(RuntimeError, match="no memory"):
+            ops.ext().cross_attention(q, q, q, None, None, None, 1, 0, 128, [])
+        with pytest.raises(RuntimeError, match="no memory"):
+            ops.ext().gated_scan(x, x, None, None, False)
