@@ -122,17 +122,26 @@ struct Items {
     const int over = max(s0 + kItems<T> - L, 0);
     const bool two = over & (2 * kEach), one = over & kEach;
     const bool half = kEach == 2 && (over & 1);
-    auto word = [&](int k) -> unsigned& { return w[REV ? 3 - k : k]; };
+    unsigned v[5];  // in scan order; values, as a choice of places is an address
 #pragma unroll
-    for (int k = 0; k < 2; ++k) word(k) = two ? word(k + 2) : word(k);
+    for (int k = 0; k < 4; ++k) v[k] = w[REV ? 3 - k : k];
+    v[4] = 0;
 #pragma unroll
-    for (int k = 0; k < 3; ++k) word(k) = one ? word(k + 1) : word(k);
+    for (int k = 0; k < 2; ++k) {
+      const unsigned here = v[k], there = v[k + 2];
+      v[k] = two ? there : here;
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const unsigned here = v[k], there = v[k + 1];
+      v[k] = one ? there : here;
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const unsigned next = k < 3 ? word(k + 1) : 0;
+      const unsigned here = v[k], next = v[k + 1];
       const unsigned moved =
-          REV ? word(k) << 16 | next >> 16 : word(k) >> 16 | next << 16;
-      word(k) = half ? moved : word(k);
+          REV ? here << 16 | next >> 16 : here >> 16 | next << 16;
+      w[REV ? 3 - k : k] = half ? moved : here;
     }
   }
   template <bool REV>
