@@ -171,13 +171,12 @@ void adam_step_packed(const at::Tensor& meta, const at::Tensor& sample,
                       double eps, double wd, double bc1, double bc2,
                       bool adamw);
 
-at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k,
-                           const at::Tensor& v,
-                           const c10::optional<at::Tensor>& lengths,
-                           const c10::optional<at::Tensor>& table,
-                           c10::optional<double> scale, long key_step,
-                           long query_start, long max_distance,
-                           std::vector<long> thresholds);
+c10::optional<at::Tensor> cross_attention(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+    const c10::optional<at::Tensor>& lengths,
+    const c10::optional<at::Tensor>& table, c10::optional<double> scale,
+    long key_step, long query_start, long max_distance,
+    std::vector<long> thresholds);
 std::vector<at::Tensor> gated_scan_run(
     const at::Tensor& x, const at::Tensor& gate,
     const c10::optional<at::Tensor>& state,

@@ -750,13 +750,17 @@ class CrossAttention : public torch::autograd::Function<CrossAttention> {
 }  // namespace
 }  // namespace attend
 
-at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k,
+// nothing where a call is recorded or a tensor only stands for one
+c10::optional<at::Tensor> cross_attention(const at::Tensor& q, const at::Tensor& k,
                            const at::Tensor& v,
                            const c10::optional<at::Tensor>& lengths,
                            const c10::optional<at::Tensor>& table,
                            c10::optional<double> scale, long key_step,
                            long query_start, long max_distance,
                            std::vector<long> thresholds) {
+  if (sa::recorded() || sa::stands_in(q) || sa::stands_in(k) ||
+      sa::stands_in(v) || sa::stands_in(lengths) || sa::stands_in(table))
+    return c10::nullopt;
   const auto call =
       attend::checked(q, k, v, lengths, table, scale, key_step, query_start,
                       max_distance, std::move(thresholds));

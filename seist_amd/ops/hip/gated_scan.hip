@@ -843,11 +843,15 @@ class GatedScan : public torch::autograd::Function<GatedScan> {
 }  // namespace
 }  // namespace gated_scan
 
-// {h, last state}
+// {h, last state}, or nothing where a call is recorded or a tensor only stands
+// for one
 std::vector<at::Tensor> gated_scan_run(
     const at::Tensor& x, const at::Tensor& gate,
     const c10::optional<at::Tensor>& state,
     const c10::optional<at::Tensor>& lengths, bool reverse) {
+  if (sa::recorded() || sa::stands_in(x) || sa::stands_in(gate) ||
+      sa::stands_in(state) || sa::stands_in(lengths))
+    return {};
   const auto call = gated_scan::checked(x, gate, state, lengths, reverse);
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || gate.requires_grad() ||

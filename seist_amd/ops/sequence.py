@@ -29,29 +29,6 @@ def _refuse(op: str, what: str):
     raise ValueError(f"{op}: {what}")
 
 
-# modes of torch that put other tensors in a call's place, or record it
-_MODES = (torch._C._TorchDispatchModeKey.FAKE,
-          torch._C._TorchDispatchModeKey.PROXY,
-          torch._C._TorchDispatchModeKey.FUNCTIONAL)
-
-
-def _runs_native(*tensors: Optional[torch.Tensor]) -> bool:
-    """Whether the kernels run: on tensors that have memory, in a call that
-    is carried out here and now. A tracer sees the extension's allocations and
-    not its launches, and a tensor that only stands for one (a fake one) has a
-    null pointer, which a kernel would write to; both are given the plain
-    steps, which they can follow."""
-    if not use_native(tensors[0]) or torch.jit.is_tracing():
-        return False
-    if torch._C._len_torch_dispatch_stack() and any(
-            torch._C._get_dispatch_mode(m) is not None for m in _MODES):
-        return False
-    return not any(
-        type(t) is not torch.Tensor and isinstance(t, torch.Tensor)
-        and torch._C._dispatch_keys(t).has(torch._C.DispatchKey.Python)
-        for t in tensors)
-
-
 def _check_lengths(op: str, name: str, lengths, like: torch.Tensor):
     if lengths is not None and (
             lengths.dim() != 1 or lengths.size(0) != like.size(0)
@@ -222,11 +199,14 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if bias_table is not None and bias_table.dim() == 2:
         _check_buckets("cross_attention", bias_table.size(1), max_distance)
         thresholds = _bucket_thresholds(bias_table.size(1), max_distance)
-    if _runs_native(q, k, v, kv_lengths, bias_table):
-        # with its own checks, the same as those below
-        return ext().cross_attention(q, k, v, kv_lengths, bias_table, scale,
-                                     key_step, query_start, max_distance,
-                                     thresholds)
+    if use_native(q):
+        # with its own checks, the same as those below; nothing where torch
+        # traces, which the plain steps can be followed by
+        out = ext().cross_attention(q, k, v, kv_lengths, bias_table, scale,
+                                    key_step, query_start, max_distance,
+                                    thresholds)
+        if out is not None:
+            return out
     _check_cross_attention(q, k, v, kv_lengths, bias_table, scale, key_step,
                            query_start)
     if scale is None:
@@ -304,9 +284,12 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor,
     zero, the state stays, and nothing is read into the result. ``reverse``
     runs from the last sample that counts to the first.
     """
-    if _runs_native(x, gate, state, lengths):
-        # with its own checks, the same as those below
-        h, last = ext().gated_scan(x, gate, state, lengths, reverse)
-        return h, last
+    if use_native(x):
+        # with its own checks, the same as those below; nothing where torch
+        # traces, which the plain steps can be followed by
+        found = ext().gated_scan(x, gate, state, lengths, reverse)
+        if found:
+            h, last = found
+            return h, last
     _check_gated_scan(x, gate, state, lengths)
     return _gated_scan_plain(x, gate, state, lengths, reverse)

@@ -152,11 +152,20 @@ def test_recorded_calls_compute_their_own_inputs():
 
 
 @pytest.mark.skipif(not ops.has_ext(), reason="the extension is not built")
-def test_the_extension_refuses_tensors_without_memory():
+def test_the_extension_leaves_recorded_and_fake_calls():
+    def nothing(q, x):
+        args = (None, None, None, 1, 0, 128, [])
+        assert ops.ext().cross_attention(q, q, q, *args) is None
+        assert not ops.ext().gated_scan(x, x, None, None, False)
+        return q * 2
+
     with FakeTensorMode():
         q = torch.empty(1, 2, 4, 5, device="cuda")
         x = torch.empty(1, 2, 5, device="cuda")
-        with pytest.raises(RuntimeError, match="no memory"):
-            ops.ext().cross_attention(q, q, q, None, None, None, 1, 0, 128, [])
-        with pytest.raises(RuntimeError, match="no memory"):
-            ops.ext().gated_scan(x, x, None, None, False)
+        nothing(q, x)
+    nothing(q, x)
+    real = _inputs((1, 2, 4, 5), (1, 2, 5))
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        nothing(*real)
+    make_fx(nothing)(*real)
+    torch.jit.trace(nothing, tuple(real), check_trace=False)
