@@ -134,7 +134,7 @@ __device__ __forceinline__ void add_diagonals(const Bias& b,
 //
 // Bound as the forward kernel is: 4096 x 4096, 64 heads of 128 on 16, 820 us,
 // 1006 TFLOP/s; (8, 8, 2048 x 1000 at most) heads of 64 with a bias 43 us for
-// DELTA and 94 for TABLE.
+// DELTA and 96 for TABLE.
 enum Find { DQ, DELTA, TABLE };
 
 template <typename T, int ED, int POS, bool LINED, Find FIND>
@@ -618,8 +618,8 @@ struct Walk {
 // Heads of up to 64 bf16 or 32 fp32 channels: a wave makes both gradients of
 // its keys, whose sums are at most 64 registers each. 256 heads of 32, 1024
 // queries to lengths up to 1024: 89 us, of which the exponentials fill 13 and
-// the products, at a large one's rate, 28; the rest are the vector
-// instructions between them.
+// the products, at a large one's rate, 28. The lengths are another part: each
+// die has 137 workgroups with keys for 64 places, three rounds for 2.1.
 template <typename T, int ED, int POS, bool LINED>
 __global__ __launch_bounds__(256, 2) void attend_dkv_kernel(Args p) {
   using M = Mma<T>;

@@ -25,8 +25,8 @@
 // twice, so it is used only where the rows alone give too few waves.
 //
 // Measured: (100, 64, 8192) bf16 67 us (4.7 TB/s) and 97 us backward (5.4
-// TB/s; a large copy reaches 5.2); one record of (24, 1000003) fp32 43 + 55
-// us in two kernels (288 MB), 40 + 105 backward (480 MB). One sample of 64 x
+// TB/s; a large copy reaches 5.2); one record of (24, 1000003) fp32 38 + 49
+// us in two kernels (288 MB), 37 + 91 backward (480 MB). One sample of 64 x
 // 96 states, a launch and no more, 3.7 us.
 
 #include <torch/extension.h>

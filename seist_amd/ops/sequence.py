@@ -177,7 +177,12 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     fp32. Any strides; a copy is made only where the last axis is not
     contiguous or a head's channels lie further apart than 4 GiB, which a
     head has to fit into. Returns (N, H, E, Lq) in q's type. ``scale``
-    defaults to 1 / sqrt(E). Differentiable in q, k, v and ``bias_table``.
+    defaults to 1 / sqrt(E). Differentiable in q, k, v and ``bias_table``,
+    once and in reverse mode; the kernels refuse other derivatives.
+
+    Scores, weights' sums and gradients are summed in 32 bits. In bf16 the
+    weights, and in the gradients their slopes, are rounded to bf16 where they
+    meet the values, keys and queries.
 
     ``kv_lengths``: (N,), the keys of each record that count, from 0 to Lk;
     nothing behind them is read into the result, NaN included.
@@ -187,11 +192,12 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ``j * key_step - (query_start + i)`` for key j and query i. ``key_step``
     is the number of query positions a key stands for (the pooling ratio of
     pooled keys), ``query_start`` the position of the first query (for queries
-    that come one at a time). An entry at or under -1e30, such as -inf or the
-    type's lowest value, takes its pairs out of the softmax whatever their
-    scores are, NaN and infinities included. Their weights are zeros, which
-    still meet the values, and in the gradients the keys and queries: only
-    what is behind ``kv_lengths`` may hold anything there.
+    that come one at a time); positions stay under 2**27. An entry at or under
+    -1e30, such as -inf or the type's lowest value, takes its pairs out of the
+    softmax whatever their scores are, NaN and infinities included. Their
+    weights are zeros, which still meet the values, and in the gradients the
+    keys and queries: only what is behind ``kv_lengths`` may hold anything
+    there.
 
     A query with no key left gives zeros and no gradient.
     """
@@ -278,7 +284,8 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor,
     state before the first sample, zeros by default. Returns h (N, C, L) in
     x's type and the fp32 state (N, C) after the last sample, which continues
     a record that comes in pieces, down to one sample a call. Differentiable
-    in x, gate and state.
+    in x, gate and state, once and in reverse mode; the kernels refuse other
+    derivatives, 2**24 rows and more, and 2**30 samples and more.
 
     ``lengths``: (N,), the samples of each record that count; behind them h is
     zero, the state stays, and nothing is read into the result. ``reverse``
