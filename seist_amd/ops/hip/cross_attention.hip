@@ -124,8 +124,7 @@ attend_kernel(Args p) {
   const int g = min(first / p.pad, p.G - 1);
   const int head = hk * p.G + g;
   const int i0 = first - g * p.pad + (lane & 31);
-  float before = 0.0f, behind = 0.0f;
-  float entry = 0.0f;
+  float before = 0.0f, behind = 0.0f, entry = 0.0f;
   if (BIASED) {  // the workgroup's rows are one head's
     entry = entry_of_lane<T>(p.bias, head);
     spread_bias<T, false>(p.bias, head, line, tid, 256);
@@ -751,13 +750,12 @@ class CrossAttention : public torch::autograd::Function<CrossAttention> {
 }  // namespace attend
 
 // nothing where a call is recorded or a tensor only stands for one
-c10::optional<at::Tensor> cross_attention(const at::Tensor& q, const at::Tensor& k,
-                           const at::Tensor& v,
-                           const c10::optional<at::Tensor>& lengths,
-                           const c10::optional<at::Tensor>& table,
-                           c10::optional<double> scale, long key_step,
-                           long query_start, long max_distance,
-                           std::vector<long> thresholds) {
+c10::optional<at::Tensor> cross_attention(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+    const c10::optional<at::Tensor>& lengths,
+    const c10::optional<at::Tensor>& table, c10::optional<double> scale,
+    long key_step, long query_start, long max_distance,
+    std::vector<long> thresholds) {
   if (sa::recorded() || sa::stands_in(q) || sa::stands_in(k) ||
       sa::stands_in(v) || sa::stands_in(lengths) || sa::stands_in(table))
     return c10::nullopt;
